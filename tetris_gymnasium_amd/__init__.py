@@ -4,5 +4,6 @@ Python host code calls hand-written HIP (gfx950) through a thin ctypes C ABI.  N
 """
 from . import _native  # noqa: F401
 from .engine import DeviceArray, Engine, EngineError  # noqa: F401
+from . import ops  # noqa: F401
 
-__all__ = ["DeviceArray", "Engine", "EngineError"]
+__all__ = ["DeviceArray", "Engine", "EngineError", "ops"]

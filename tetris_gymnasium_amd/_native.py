@@ -26,6 +26,7 @@ OUT_COMMITTED, OUT_ILLEGAL = 1, 2  # tg_step_out.flags
 NONE = 0xFF
 OK, EINVAL, EHIP, ENOMEM, EUNSUPPORTED = 0, -1, -2, -3, -4  # TG_E*
 F_GAME_OVER, F_HAS_SWAPPED, F_PENDING_RESET = 1, 2, 4
+T_U8, T_I8, T_F32, T_F16, T_BF16 = range(5)  # include/tetris_gym_ops.h element types
 
 ENV_REC = np.dtype(
     [
@@ -107,6 +108,21 @@ SYMBOLS = {
     "tg_stream_copy_gbps": (_i, [_vp, _sz, _i, C.POINTER(C.c_float)]),
     "tg_shape_mask": (_i, [_i, _i]),
 }
+
+# include/tetris_gym_ops.h: the operators between observations and actions.  The product library holds them; a library given with TG_LIB
+# that implements tetris_gym_hip.h alone (the CPU checker's) loads without them and ops.py refuses its calls.
+_i64, _pp = C.c_int64, C.POINTER(_vp)
+OPS_SYMBOLS = {
+    "tg_ops_last_error": (C.c_char_p, []),
+    "tg_linear_i8": (_i, [_i, _vp, _vp, _i, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i, _vp, _i, _i64]),
+    "tg_quantize_i8": (_i, [_i, _vp, _vp, _i, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "tg_beam_select_workspace": (_i64, [_i64] * 4),
+    "tg_beam_select": (_i, [_i, _vp, _vp, _i] + [_i64] * 5 + [_vp, _vp, _i64, _i64, _vp, _i, _i, _i64, _vp, _vp, _vp, _vp, _i64]),
+    "tg_beam_reorder": (_i, [_i, _vp, _i, _pp, _pp, C.POINTER(_i64), C.POINTER(_i64), C.POINTER(_i64), _i64, _i64, _i64, _vp]),
+    "tg_reorder_beams": (_i, [_vp, _vp, _i]),
+    "tg_stream": (_i, [_vp, _pp]),
+}
+HAVE_OPS = False
 
 _lib = None
 
@@ -200,7 +216,7 @@ def _needed_hip_soname(path):
 
 def load() -> C.CDLL:
     """Load the HIP engine.  Raises NativeLibraryError (never falls back) when it is unavailable."""
-    global _lib
+    global _lib, HAVE_OPS
     if _lib is not None:
         return _lib
     if not os.path.exists(LIB_PATH):
@@ -223,6 +239,11 @@ def load() -> C.CDLL:
         fn.argtypes = args
     if lib.tg_abi_version() != ABI_VERSION:
         raise NativeLibraryError("libtetris_gym_hip.so ABI version mismatch")
+    HAVE_OPS = all(hasattr(lib, name) for name in OPS_SYMBOLS)
+    for name, (res, args) in OPS_SYMBOLS.items() if HAVE_OPS else ():
+        fn = getattr(lib, name)
+        fn.restype = res
+        fn.argtypes = args
     _lib = lib
     if os.environ.get("TG_VERBOSE"):
         import sys

@@ -27,6 +27,7 @@
 #include <thread>
 #include <vector>
 
+#include "../../include/tetris_gym_ops.h"
 #include "tg_kernel_bits.h"
 #include "tg_kernel_features.h"
 #include "tg_kernel_placements.h"
@@ -2179,6 +2180,62 @@ int tg_features(tg_handle* h) {
   HIPCHK(h, hipGetLastError());
   return TG_OK;
 }
+
+#ifndef TG_LEGACY_KERNELS  // (the operators are not part of the test-only legacy library)
+int tg_stream(tg_handle* h, void** stream) {
+  if (!h || !stream) return TG_EINVAL;
+  HIPCHK(h, hipSetDevice(h->cfg.device));
+  { int rcj = join_shards(h); if (rcj != TG_OK) return rcj; }
+  *stream = h->stream;
+  return TG_OK;
+}
+
+// Every array a transition reads or a caller sees is one row per env (the double-buffered ones: one row per env and parity), so the
+// state of the whole handle moves in one launch.  What is derived on demand (legal mask, host pack, features) is not state, and
+// a packed handle's stale uint8 board stays as stale as it was.
+int tg_reorder_beams(tg_handle* h, const int32_t* parents, int beams) {
+  if (!h) return TG_EINVAL;
+  if (!parents) return fail(h, TG_EINVAL, "tg_reorder_beams: null parents");
+  if (beams < 1 || beams > TG_OPS_MAX_BEAMS || h->B % beams)
+    return fail(h, TG_EINVAL, "tg_reorder_beams: %d beams: 1 .. %d that divide the batch of %d are supported", beams, TG_OPS_MAX_BEAMS, h->B);
+  if (const void* z = std::memchr(h->rng_valid.data(), 0, (size_t)h->B))
+    return fail(h, TG_EINVAL, "tg_reorder_beams: env %d was never reset", (int)((const uint8_t*)z - h->rng_valid.data()));
+  HIPCHK(h, hipSetDevice(h->cfg.device));
+  { int rcj = join_shards(h); if (rcj != TG_OK) return rcj; }
+  void* at[TG_OPS_MAX_STATES];
+  int64_t bytes[TG_OPS_MAX_STATES];
+  int n = 0;
+  const size_t B = (size_t)h->B;
+  auto add = [&](void* p, size_t row) {
+    if (p && row) { at[n] = p; bytes[n++] = (int64_t)row; }
+  };
+  if (h->cfg.obs_mode == TG_OBS_DICT) {  // (four arrays behind each other)
+    const size_t pc = (size_t)(h->W + 8) * (h->H + 4), parts[4] = {pc, pc, 16, 16 * (size_t)h->Q};
+    uint8_t* p = (uint8_t*)h->buf[TG_BUF_OBS];
+    for (size_t r : parts) { add(p, r); p += B * r; }
+  } else {
+    add(h->buf[TG_BUF_OBS], obs_bytes_per_env(&h->cfg));
+  }
+  for (int which : {TG_BUF_STEP_OUT, TG_BUF_BOARD, TG_BUF_REC, TG_BUF_RNG, TG_BUF_FINAL_OBS, TG_BUF_EPISODE})
+    if (h->bytes[which]) add(h->buf[which], h->bytes[which] / B);
+  add(h->d_pboard, h->cells / 2);
+  if (h->d_cols) {
+    add(h->d_cols, h->L.cols_bytes);
+    add(h->d_ahead, 32 * tg::kRing);
+    if (h->cfg.ruleset == TG_RULESET_NUMPY) {
+      for (size_t parity = 0; parity < 2; ++parity) {
+        add((uint8_t*)h->d_ring + parity * B * 16, 16);
+        add((uint8_t*)h->d_hbuf + parity * B * 4, 4);
+        add((uint8_t*)h->d_inl + parity * B * 32, 32);
+      }
+    } else {
+      add(h->d_hbuf, 8);
+    }
+  }
+  const int rc = tg_beam_reorder(h->cfg.device, h->stream, n, at, at, bytes, bytes, bytes, h->B / beams, beams, beams, parents);
+  return rc == TG_OK ? TG_OK : fail(h, rc, "tg_reorder_beams: %s", tg_ops_last_error());
+}
+#endif
 
 int tg_sync(tg_handle* h) {
   if (!h) return TG_EINVAL;

@@ -1,0 +1,259 @@
+// Host side of the operators' C ABI (include/tetris_gym_ops.h): checks, choice of a kernel, launch.
+#include <cstdarg>
+#include <cstdio>
+#include <cstring>
+
+#include "../../include/tetris_gym_hip.h"
+#include "../../include/tetris_gym_ops.h"
+#include "tg_op_beam.h"
+#include "tg_op_linear.h"
+#include "tg_op_quantize.h"
+
+using namespace tg::ops;
+
+namespace {
+
+thread_local char g_err[512];
+
+int fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+// the call's device for the duration of the call
+struct DeviceScope {
+  int before = -1;
+  hipError_t err;
+  explicit DeviceScope(int device) {
+    err = hipGetDevice(&before);
+    if (err == hipSuccess && before != device) err = hipSetDevice(device);
+    else before = -1;
+  }
+  ~DeviceScope() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+#define ON_DEVICE(name, device)                                                                             \
+  DeviceScope scope(device);                                                                                \
+  if (scope.err != hipSuccess) {                                                                            \
+    (void)hipGetLastError();                                                                                \
+    return fail(TG_EHIP, name ": device %d: %s (there is no CPU fallback)", device, hipGetErrorString(scope.err)); \
+  }
+
+int launched(const char* name) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? TG_OK : fail(TG_EHIP, "%s: launch failed: %s", name, hipGetErrorString(e));
+}
+
+int type_size(int t) { return t <= kI8 ? 1 : t == kF32 ? 4 : 2; }
+bool is_float(int t) { return t == kF32 || t == kF16 || t == kBF16; }
+
+// bytes from the first to behind the last element of [rows][cols] with a row stride (rows, cols > 0)
+int64_t span(int64_t rows, int64_t cols, int64_t stride, int64_t size) { return ((rows - 1) * stride + cols) * size; }
+bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+  return a && b && (const char*)a < (const char*)b + nb && (const char*)b < (const char*)a + na;
+}
+constexpr int64_t kMost = (int64_t)1 << 40;  // sizes and strides beyond a card's memory: products of two stay in 64 bits below
+constexpr int64_t kMaxGrid = 0x7FFFFFFF;
+
+template <class F> int by_float(int t, F f) {
+  if (t == kF32) return f(float{});
+  if (t == kF16) return f(_Float16{});
+  return f(bf16_t{});
+}
+
+}  // namespace
+
+extern "C" {
+
+const char* tg_ops_last_error(void) { return g_err; }
+
+int tg_linear_i8(int device, void* stream, const void* x, int x_type, int64_t rows, int64_t k, int64_t x_stride, const int8_t* w, int64_t n,
+                 int64_t w_stride, const float* w_scale, const float* x_scale, const float* bias, int relu, void* out, int out_type,
+                 int64_t out_stride) {
+  if (x_type != kU8 && x_type != kI8) return fail(TG_EINVAL, "tg_linear_i8: x must be u8 or i8, got type %d", x_type);
+  if (!is_float(out_type)) return fail(TG_EINVAL, "tg_linear_i8: out must be f32, f16 or bf16, got type %d", out_type);
+  if (rows < 0 || n < 0 || k < 0 || rows > kMost || n > kMost) return fail(TG_EINVAL, "tg_linear_i8: bad sizes (rows %lld, k %lld, n %lld)", (long long)rows, (long long)k, (long long)n);
+  if (k > TG_OPS_MAX_K) return fail(TG_EINVAL, "tg_linear_i8: k = %lld, the 32-bit sum is exact up to %d", (long long)k, TG_OPS_MAX_K);
+  if (rows == 0 || n == 0) return TG_OK;
+  if ((rows > 1 && (x_stride < 0 || x_stride > (1 << 24))) || (n > 1 && (w_stride < k || w_stride > (1 << 24))))
+    return fail(TG_EINVAL, "tg_linear_i8: row strides (x %lld, w %lld) out of range", (long long)x_stride, (long long)w_stride);
+  if (rows > 1 && (out_stride < n || out_stride > (1 << 24))) return fail(TG_EINVAL, "tg_linear_i8: the output's row stride %lld must be n .. 2^24", (long long)out_stride);
+  if (n > (1 << 24) || rows > ((int64_t)1 << 34)) return fail(TG_EINVAL, "tg_linear_i8: n = %lld or rows = %lld too large", (long long)n, (long long)rows);
+  if (!out || !w_scale || (k && (!x || !w))) return fail(TG_EINVAL, "tg_linear_i8: null pointer");
+  const int os = type_size(out_type);
+  if ((uintptr_t)out % os || (uintptr_t)w_scale % 4 || (uintptr_t)x_scale % 4 || (uintptr_t)bias % 4)
+    return fail(TG_EINVAL, "tg_linear_i8: out / w_scale / x_scale / bias not aligned to their elements");
+  if (rows == 1) { x_stride = k; out_stride = n; }
+  if (n == 1) w_stride = k;
+  const int64_t no = span(rows, n, out_stride, os);
+  if ((k && (overlap(out, no, x, span(rows, k, x_stride, 1)) || overlap(out, no, w, span(n, k, w_stride, 1)))) || overlap(out, no, w_scale, 4 * n) ||
+      overlap(out, no, x_scale, 4 * rows) || overlap(out, no, bias, 4 * n))
+    return fail(TG_EINVAL, "tg_linear_i8: the output overlaps an input");
+  ON_DEVICE("tg_linear_i8", device);
+  LinearArgs a{(const uint8_t*)x, w, w_scale, x_scale, bias, out, rows, k, n, x_stride, w_stride, out_stride, relu != 0,
+               (uintptr_t)out % 16 == 0 && (out_stride * os) % 16 == 0};
+  by_float(out_type, [&](auto o) {
+    using OT = decltype(o);
+    // (grid.x holds rows: 2^34 / 64 workgroups; grid.y columns: 2^24 / 64 would pass 65 535, so wide outputs go in parts)
+    for (int64_t c = 0; c < n; c += 65535 * 64) {
+      LinearArgs b = a;
+      b.w = w + c * w_stride;
+      b.ws = w_scale + c;
+      b.bias = bias ? bias + c : nullptr;
+      b.out = (OT*)out + c;
+      b.n = n - c < 65535 * 64 ? n - c : 65535 * 64;
+      const dim3 grid((unsigned)((rows + 63) / 64), (unsigned)((b.n + 63) / 64));
+      if (x_type == kU8) hipLaunchKernelGGL((linear_wave_kernel<OT, true>), grid, dim3(256), 0, (hipStream_t)stream, b);
+      else hipLaunchKernelGGL((linear_wave_kernel<OT, false>), grid, dim3(256), 0, (hipStream_t)stream, b);
+    }
+    return 0;
+  });
+  return launched("tg_linear_i8");
+}
+
+int tg_quantize_i8(int device, void* stream, const void* x, int x_type, int64_t rows, int64_t k, int64_t x_stride, int8_t* q, int64_t q_stride,
+                   float* scale) {
+  if (!is_float(x_type)) return fail(TG_EINVAL, "tg_quantize_i8: x must be f32, f16 or bf16, got type %d", x_type);
+  if (rows < 0 || k < 0 || rows > ((int64_t)1 << 34) || k > (1 << 30)) return fail(TG_EINVAL, "tg_quantize_i8: bad sizes (rows %lld, k %lld)", (long long)rows, (long long)k);
+  if (rows == 0) return TG_OK;
+  if (rows > 1 && (x_stride < 0 || x_stride > (1 << 30) || q_stride < k || q_stride > (1 << 30)))
+    return fail(TG_EINVAL, "tg_quantize_i8: row strides (x %lld, q %lld) out of range", (long long)x_stride, (long long)q_stride);
+  if (!scale || (k && (!x || !q))) return fail(TG_EINVAL, "tg_quantize_i8: null pointer");
+  const int size = type_size(x_type);
+  if ((uintptr_t)x % size || (uintptr_t)scale % 4) return fail(TG_EINVAL, "tg_quantize_i8: x / scale not aligned to their elements");
+  if (rows == 1) { x_stride = k; q_stride = k; }
+  if (k) {
+    const int64_t nx = span(rows, k, x_stride, size), nq = span(rows, k, q_stride, 1);
+    if (overlap(q, nq, x, nx) || overlap(scale, 4 * rows, x, nx) || overlap(scale, 4 * rows, q, nq))
+      return fail(TG_EINVAL, "tg_quantize_i8: the outputs overlap each other or the input");
+  }
+  ON_DEVICE("tg_quantize_i8", device);
+  by_float(x_type, [&](auto e) {
+    using T = decltype(e);
+    const int64_t vec = kQVec<T>;
+    const auto grid = [&](int rpb) { return dim3((unsigned)((rows + rpb - 1) / rpb)); };
+    if (k <= 16 * 4 * vec) hipLaunchKernelGGL((quantize_kernel<T, 16, 4>), grid(16), dim3(256), 0, (hipStream_t)stream, (const T*)x, rows, k, x_stride, q, q_stride, scale);
+    else if (k <= 64 * 4 * vec) hipLaunchKernelGGL((quantize_kernel<T, 64, 4>), grid(4), dim3(256), 0, (hipStream_t)stream, (const T*)x, rows, k, x_stride, q, q_stride, scale);
+    else {
+      for (int64_t r = 0; r < rows; r += kMaxGrid) {
+        const int64_t c = rows - r < kMaxGrid ? rows - r : kMaxGrid;
+        hipLaunchKernelGGL((quantize_kernel<T, 256, 4>), dim3((unsigned)c), dim3(256), 0, (hipStream_t)stream, (const T*)x + r * x_stride, c, k,
+                           x_stride, q + r * q_stride, q_stride, scale + r);
+      }
+    }
+    return 0;
+  });
+  return launched("tg_quantize_i8");
+}
+
+int64_t tg_beam_select_workspace(int64_t groups, int64_t beams_in, int64_t vocab, int64_t beams_out) {
+  if (groups < 0 || beams_in < 0 || vocab < 0 || beams_out < 0) return fail(TG_EINVAL, "tg_beam_select_workspace: negative size");
+  return 0;
+}
+
+int tg_beam_select(int device, void* stream, const void* logits, int type, int64_t groups, int64_t beams_in, int64_t vocab, int64_t lg,
+                   int64_t lk, const float* scores, const uint8_t* mask, int64_t mg, int64_t mk, const uint8_t* finished, int pad,
+                   int normalize, int64_t beams_out, float* out_scores, int32_t* parents, int32_t* tokens, void* workspace,
+                   int64_t workspace_bytes) {
+  if (!is_float(type)) return fail(TG_EINVAL, "tg_beam_select: logits must be f32, f16 or bf16, got type %d", type);
+  if (groups < 0 || groups > kMaxGrid) return fail(TG_EINVAL, "tg_beam_select: %lld groups", (long long)groups);
+  if (beams_in < 1 || beams_in > TG_OPS_MAX_BEAMS || beams_out < 1 || beams_out > TG_OPS_MAX_BEAMS)
+    return fail(TG_EINVAL, "tg_beam_select: %lld beams in, %lld out: 1 .. %d are supported", (long long)beams_in, (long long)beams_out, TG_OPS_MAX_BEAMS);
+  if (vocab < 1 || vocab > (1 << 24)) return fail(TG_EINVAL, "tg_beam_select: %lld entries: 1 .. 2^24 are supported", (long long)vocab);
+  if (finished && (pad < 0 || pad >= vocab)) return fail(TG_EINVAL, "tg_beam_select: pad %d outside the %lld entries", pad, (long long)vocab);
+  if (groups == 0) return TG_OK;
+  if (lg < 0 || lk < 0 || lg > kMost || lk > kMost / 64 || (mask && (mg < 0 || mk < 0 || mg > kMost || mk > kMost / 64)))
+    return fail(TG_EINVAL, "tg_beam_select: negative or too large strides");
+  if (!logits || !scores || !out_scores || !parents || !tokens) return fail(TG_EINVAL, "tg_beam_select: null pointer");
+  if ((uintptr_t)logits % type_size(type) || (uintptr_t)scores % 4 || (uintptr_t)out_scores % 4 || (uintptr_t)parents % 4 || (uintptr_t)tokens % 4)
+    return fail(TG_EINVAL, "tg_beam_select: an array is not aligned to its elements");
+  const int64_t need = tg_beam_select_workspace(groups, beams_in, vocab, beams_out);
+  if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+    return fail(TG_EINVAL, "tg_beam_select: a 16-byte aligned workspace of %lld bytes is needed, got %lld", (long long)need, (long long)workspace_bytes);
+  {
+    const int64_t no = 4 * groups * beams_out, ni = 4 * groups * beams_in;
+    const int64_t nl = ((groups - 1) * lg + (beams_in - 1) * lk + vocab) * type_size(type), nm = (groups - 1) * mg + (beams_in - 1) * mk + vocab;
+    const void* outs[3] = {out_scores, parents, tokens};
+    for (int i = 0; i < 3; ++i) {
+      if (overlap(outs[i], no, logits, nl) || overlap(outs[i], no, scores, ni) || (mask && overlap(outs[i], no, mask, nm)) ||
+          overlap(outs[i], no, finished, ni / 4) || overlap(outs[i], no, outs[(i + 1) % 3], no) || (need && overlap(outs[i], no, workspace, need)))
+        return fail(TG_EINVAL, "tg_beam_select: the outputs overlap each other or an input");
+    }
+  }
+  ON_DEVICE("tg_beam_select", device);
+  const SelectArgs a{logits, scores, mask, finished, out_scores, parents, tokens, lg, lk, mg, mk, groups, (int)beams_in, (int)vocab, (int)beams_out, pad, normalize != 0};
+  by_float(type, [&](auto e) {
+    using T = decltype(e);
+    hipLaunchKernelGGL((select_scan_kernel<T>), dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, a);
+    return 0;
+  });
+  return launched("tg_beam_select");
+}
+
+int tg_beam_reorder(int device, void* stream, int n, const void* const* src, void* const* dst, const int64_t* row_bytes,
+                    const int64_t* src_stride, const int64_t* dst_stride, int64_t groups, int64_t beams_in, int64_t beams_out,
+                    const int32_t* parents) {
+  if (n < 0 || n > TG_OPS_MAX_STATES) return fail(TG_EINVAL, "tg_beam_reorder: %d arrays: up to %d go into one call", n, TG_OPS_MAX_STATES);
+  if (groups < 0 || groups > kMaxGrid) return fail(TG_EINVAL, "tg_beam_reorder: %lld groups", (long long)groups);
+  if (beams_in < 1 || beams_in > TG_OPS_MAX_BEAMS || beams_out < 1 || beams_out > TG_OPS_MAX_BEAMS)
+    return fail(TG_EINVAL, "tg_beam_reorder: %lld beams in, %lld out: 1 .. %d are supported", (long long)beams_in, (long long)beams_out, TG_OPS_MAX_BEAMS);
+  if (n == 0 || groups == 0) return TG_OK;
+  if (!src || !dst || !row_bytes || !src_stride || !dst_stride || !parents) return fail(TG_EINVAL, "tg_beam_reorder: null pointer");
+  if ((uintptr_t)parents % 4) return fail(TG_EINVAL, "tg_beam_reorder: parents not aligned");
+  ReorderArgs p{};
+  const int64_t rin = groups * beams_in, rout = groups * beams_out;
+  bool in_place = dst[0] == src[0];
+  for (int i = 0; i < n; ++i) {
+    const int64_t rb = row_bytes[i], ss = src_stride[i], ds = dst_stride[i];
+    if (rb < 0 || rb > kMost || ss < rb || ds < rb || ss > kMost / 64 || ds > kMost / 64)
+      return fail(TG_EINVAL, "tg_beam_reorder: array %d: rows of %lld bytes at strides %lld / %lld", i, (long long)rb, (long long)ss, (long long)ds);
+    if (rb == 0) continue;
+    if (!src[i] || !dst[i]) return fail(TG_EINVAL, "tg_beam_reorder: array %d is null", i);
+    const int64_t ns = (rin - 1) * ss + rb, nd = (rout - 1) * ds + rb;
+    if (overlap(dst[i], nd, parents, 4 * rout)) return fail(TG_EINVAL, "tg_beam_reorder: array %d overlaps the parents", i);
+    if ((dst[i] == src[i]) != in_place) return fail(TG_EINVAL, "tg_beam_reorder: some arrays in place and some not");
+    if (in_place && (ss != ds || beams_in != beams_out)) return fail(TG_EINVAL, "tg_beam_reorder: array %d: in place needs equal strides and beams", i);
+    for (int j = 0; j < n; ++j) {
+      if (row_bytes[j] <= 0 || (in_place && j == i)) continue;
+      if (overlap(dst[i], nd, src[j], (rin - 1) * src_stride[j] + row_bytes[j]) ||
+          (j != i && overlap(dst[i], nd, dst[j], (rout - 1) * dst_stride[j] + row_bytes[j])))
+        return fail(TG_EINVAL, "tg_beam_reorder: arrays %d and %d overlap", i, j);
+    }
+    (void)ns;
+    ReorderArray& a = p.a[p.n];
+    a.src = (const uint8_t*)src[i];
+    a.dst = (uint8_t*)dst[i];
+    a.src_stride = ss;
+    a.dst_stride = ds;
+    const uint64_t bits = (uint64_t)(uintptr_t)src[i] | (uintptr_t)dst[i] | (uint64_t)rb | (uint64_t)ss | (uint64_t)ds | 16;
+    a.shift = __builtin_ctzll(bits);
+    a.units = rb >> a.shift;
+    const int64_t most = 64 * kReorderReg / beams_out;  // columns of an item of one group
+    a.cb = (int)(a.units < most ? a.units : most);
+    a.gp = (int)(64 * kReorderReg / (beams_out * a.cb));
+    if (a.cb < a.units) a.gp = 1;
+    a.mul_cb = ((1u << 20) + a.cb - 1) / a.cb;
+    a.mul_out = ((1u << 20) + (uint32_t)beams_out - 1) / (uint32_t)beams_out;
+    const int64_t blocks = (a.units + a.cb - 1) / a.cb, items = blocks * ((groups + a.gp - 1) / a.gp);
+    if (blocks > kMaxGrid || items + p.items > kMaxGrid) return fail(TG_EINVAL, "tg_beam_reorder: too much in one call (array %d)", i);
+    a.blocks = (uint32_t)blocks;
+    a.first = p.items;
+    p.items += (uint32_t)items;
+    ++p.n;
+  }
+  if (p.n == 0) return TG_OK;
+  p.parents = parents;
+  p.groups = groups;
+  p.kin = (int)beams_in;
+  p.kout = (int)beams_out;
+  p.in_place = in_place;
+  ON_DEVICE("tg_beam_reorder", device);
+  hipLaunchKernelGGL(reorder_kernel, dim3((p.items + 3) / 4), dim3(256), 0, (hipStream_t)stream, p);
+  return launched("tg_beam_reorder");
+}
+
+}  // extern "C"

@@ -520,6 +520,53 @@ class Engine:
         p = [None if b is None else C.c_void_p(b.ptr if isinstance(b, DeviceBuffer) else int(b)) for b in (board, rec, rng)]
         self._chk(self.lib.tg_set_state_dev(self.h, *p), "tg_set_state_dev")
 
+    # -- searches that branch (include/tetris_gym_ops.h, ops.py, search.py) ------------------------
+    @property
+    def stream(self):
+        """The engine's HIP stream as an integer: operators called with `stream=engine.stream` run in order with its transitions."""
+        self._need_ops()
+        p = C.c_void_p()
+        self._chk(self.lib.tg_stream(self.h, C.byref(p)), "tg_stream")
+        return p.value
+
+    def reorder_beams(self, parents, beams):
+        """Env g * beams + j becomes a copy of env g * beams + parents[g, j] in every respect — board, record, generator, observation,
+        last outputs, episode statistics —, in place and asynchronous (tg_reorder_beams).  parents: int32 device memory of `batch`
+        entries (an integer pointer, a DeviceBuffer or any device array, as ops.beam_select leaves it, written in order with the
+        engine's stream) or a host array; an entry outside 0 .. beams - 1 leaves its env alone."""
+        self._need_ops()
+        beams = int(beams)
+        if beams < 1 or self.B % beams:
+            raise ValueError(f"{beams} beams do not divide the batch of {self.B}")
+        buf = None
+        if isinstance(parents, DeviceBuffer):
+            if parents.nbytes < 4 * self.B:
+                raise ValueError(f"parents: {self.B} int32 are needed, the buffer holds {parents.nbytes} bytes")
+            ptr = parents.ptr
+        elif isinstance(parents, (int, np.integer)):
+            ptr = int(parents)
+        elif isinstance(parents, (list, tuple, np.ndarray)):
+            a = np.asarray(parents)
+            if a.size != self.B or a.dtype.kind not in "iu":
+                raise ValueError(f"parents must hold {self.B} integers, got {a.dtype} {a.shape}")
+            buf = DeviceBuffer(self, 4 * self.B)
+            self.dev_upload(buf.ptr, np.clip(a.reshape(-1), -1, 2**31 - 1).astype(np.int32))
+            ptr = buf.ptr
+        else:
+            from . import ops
+
+            ptr, shape, strides, name, dev = ops._view(parents, "parents")
+            n = int(np.prod(shape, dtype=np.int64))
+            if name != "int32" or n != self.B or (dev is not None and dev != self.cfg.device):
+                raise ValueError(f"parents must be int32 [{self.B}] on device {self.cfg.device}, got {name} {tuple(shape)} on {dev}")
+            ops._dense(shape, strides, shape, "parents")
+        self._chk(self.lib.tg_reorder_beams(self.h, C.c_void_p(ptr), beams), "tg_reorder_beams")
+        del buf  # (back to the free list: whoever takes it next writes it in order with the engine's stream)
+
+    def _need_ops(self):
+        if not N.HAVE_OPS:
+            raise EngineError(f"{N.LIB_PATH} holds no operators (include/tetris_gym_ops.h)")
+
     # -- grouped action surface (wrappers/grouped.py) ---------------------------------------------
     def legal_mask(self):
         """u8 [B, 4*W]: 1 = legal placement (column*4 + rotations) for the current active pieces."""

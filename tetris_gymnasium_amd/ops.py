@@ -1,0 +1,344 @@
+"""Operators between the engine's observations and its actions, on device memory (include/tetris_gym_ops.h):
+
+* `linear_i8`    8-bit observations (or quantised activations) times 8-bit weights, scaled per row and per column
+* `quantize_i8`  rows of activations to 8 bits with one scale each — what a second layer takes
+* `beam_select`  the best continuations of a group of beams over all entries, under a legal mask
+* `beam_reorder` the rows of any number of states that follow their beams
+
+Arrays are device memory of one GPU: a PyTorch tensor, a `DeviceArray` of an Engine, anything with
+`__cuda_array_interface__`, or a `DeviceView` around a raw pointer.  Outputs are the caller's; nothing is allocated, kept or
+waited for.  Calls run on `stream` (an integer hipStream_t, e.g. `torch.cuda.current_stream().cuda_stream`; 0 = the default
+stream) in order with whatever else runs there, and may be captured into a graph.  A `DeviceArray` is exported as to any other
+consumer: its engine's stream is waited for first.  Bad arguments raise ValueError, a failed call EngineError."""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import _native as N
+from .engine import DeviceArray, EngineError
+
+MAX_BEAMS, MAX_STATES, MAX_K = 64, 24, 65536  # TG_OPS_MAX_*
+
+_TYPES = {"uint8": N.T_U8, "bool": N.T_U8, "int8": N.T_I8, "float32": N.T_F32, "float16": N.T_F16, "bfloat16": N.T_BF16, "int32": -1}
+_SIZES = {"uint8": 1, "bool": 1, "int8": 1, "float32": 4, "float16": 2, "bfloat16": 2, "int32": 4, "int64": 8, "int16": 2,
+          "float64": 8, "uint16": 2, "uint32": 4, "uint64": 8}
+_STR = {"|u1": "uint8", "|b1": "bool", "|i1": "int8", "<f4": "float32", "<f2": "float16", "<i4": "int32", "<i8": "int64", "<i2": "int16",
+        "<f8": "float64", "<u2": "uint16", "<u4": "uint32", "<u8": "uint64"}
+_names: dict = {}  # dtype object → its name
+
+
+class DeviceView:
+    """A raw device pointer with a shape: dtype by name ("uint8", "int8", "bool", "int32", "float32", "float16", "bfloat16", ...),
+    strides in elements (None = contiguous).  The caller keeps the memory alive."""
+
+    __slots__ = ("ptr", "shape", "dtype", "strides", "device")
+
+    def __init__(self, ptr, shape, dtype, strides=None, device=0):
+        if dtype not in _SIZES:
+            raise ValueError(f"DeviceView: unknown dtype {dtype!r}")
+        self.ptr, self.shape, self.dtype, self.device = int(ptr), tuple(int(n) for n in shape), dtype, int(device)
+        self.strides = _contiguous(self.shape) if strides is None else tuple(int(s) for s in strides)
+        if len(self.strides) != len(self.shape):
+            raise ValueError("DeviceView: one stride per axis")
+
+
+def _contiguous(shape):
+    st, n = [], 1
+    for s in reversed(shape):
+        st.append(n)
+        n *= s
+    return tuple(reversed(st))
+
+
+def _view(a, what):
+    """(pointer, shape, strides in elements, dtype name, device or None)"""
+    if hasattr(a, "data_ptr"):  # a torch tensor (not imported here)
+        dt = a.dtype
+        name = _names.get(dt)
+        if name is None:
+            name = _names[dt] = str(dt).rpartition(".")[2]
+        dev = a.device
+        if dev.type != "cuda":
+            raise ValueError(f"{what}: device memory is needed, got a tensor on {dev}")
+        return a.data_ptr(), tuple(a.shape), a.stride(), name, dev.index
+    if isinstance(a, DeviceView):
+        return a.ptr, a.shape, a.strides, a.dtype, a.device
+    if isinstance(a, DeviceArray):
+        a._ready()
+        name, item = a.dtype.name, a.dtype.itemsize
+        if a.strides is None:
+            st = _contiguous(a.shape)
+        else:
+            if any(s % item for s in a.strides):
+                raise ValueError(f"{what}: strides are not whole elements")
+            st = tuple(s // item for s in a.strides)
+        return a.ptr, a.shape, st, name, int(a.engine.cfg.device)
+    cai = getattr(a, "__cuda_array_interface__", None)
+    if cai is None:
+        raise ValueError(f"{what}: a device array is needed (torch tensor, DeviceArray, DeviceView or __cuda_array_interface__), got {type(a).__name__}")
+    name = _STR.get(cai["typestr"])
+    if name is None:
+        raise ValueError(f"{what}: unsupported element type {cai['typestr']}")
+    shape, item = tuple(cai["shape"]), _SIZES[name]
+    st = cai.get("strides")
+    st = _contiguous(shape) if st is None else tuple(s // item for s in st)
+    return cai["data"][0], shape, st, name, None
+
+
+def _device(*devs):
+    seen = {d for d in devs if d is not None}
+    if len(seen) > 1:
+        raise ValueError(f"arrays on different devices: {sorted(seen)}")
+    return seen.pop() if seen else 0
+
+
+def _lib():
+    lib = N.load()
+    if not N.HAVE_OPS:
+        raise EngineError(f"{N.LIB_PATH} holds no operators (include/tetris_gym_ops.h): build the product library")
+    return lib
+
+
+def _check(lib, rc, what):
+    if rc != N.OK:
+        msg = f"{what} failed ({rc}): {lib.tg_ops_last_error().decode()}"
+        raise ValueError(msg) if rc == N.EINVAL else EngineError(msg)
+
+
+def _type(name, what, allowed):
+    if name not in allowed:
+        raise ValueError(f"{what} must be {' / '.join(allowed)}, got {name}")
+    return _TYPES[name]
+
+
+_FLOATS = ("float32", "float16", "bfloat16")
+
+
+def _inner(shape, st, what):
+    if shape and shape[-1] > 1 and st[-1] != 1:
+        raise ValueError(f"{what}: the last axis must be contiguous")
+
+
+def _dense(shape, st, want, what):
+    """an array of exactly this shape, contiguous"""
+    if tuple(shape) != tuple(want):
+        raise ValueError(f"{what} must have shape {tuple(want)}, got {tuple(shape)}")
+    n = 1
+    for s, k in zip(reversed(st), reversed(shape)):
+        if k > 1 and s != n:
+            raise ValueError(f"{what} must be contiguous")
+        n *= k
+
+
+def _rows(shape, st, what):
+    """(rows, columns, row stride) of an array whose leading axes flatten into one"""
+    if len(shape) < 2:
+        raise ValueError(f"{what} must have at least two axes, got {shape}")
+    _inner(shape, st, what)
+    rows, stride = 1, 0
+    for s, k in zip(reversed(st[:-1]), reversed(shape[:-1])):
+        if k == 1:
+            continue
+        if rows == 1:
+            stride = s
+        elif s != stride * rows:
+            raise ValueError(f"{what}: the leading axes (shape {shape}, strides {tuple(st)}) do not flatten into rows")
+        rows *= k
+    return rows, shape[-1], stride if rows > 1 else shape[-1]
+
+
+def linear_i8(x, weight, weight_scale, out, *, x_scale=None, bias=None, relu=False, stream=0):
+    """out[..., n] = act((sum_k x[..., k] * weight[n, k]) * (x_scale[...] * weight_scale[n]) + bias[n])
+
+    x uint8 / int8 [..., K] (rows at any stride and alignment: the engine's boards and feature vectors as they lie), weight int8
+    [N, K], weight_scale float32 [N], x_scale float32 [rows] or None (1), bias float32 [N] or None, out float32 / float16 /
+    bfloat16 [..., N].  The sum is exact (K <= 65 536), the rest float32, rounded once; `relu` clips at zero.  Returns out."""
+    xp, xsh, xst, xt, d0 = _view(x, "linear_i8: x")
+    wp, wsh, wst, wt, d1 = _view(weight, "linear_i8: weight")
+    sp, ssh, sst, stt, d2 = _view(weight_scale, "linear_i8: weight_scale")
+    op, osh, ost, ot, d3 = _view(out, "linear_i8: out")
+    xtype = _type(xt, "linear_i8: x", ("uint8", "int8"))
+    _type(wt, "linear_i8: weight", ("int8",))
+    _type(stt, "linear_i8: weight_scale", ("float32",))
+    otype = _type(ot, "linear_i8: out", _FLOATS)
+    rows, k, xs = _rows(xsh, xst, "linear_i8: x")
+    orows, n, os_ = _rows(osh, ost, "linear_i8: out")
+    if len(wsh) != 2 or wsh != (n, k):
+        raise ValueError(f"linear_i8: weight must have shape {(n, k)}, got {tuple(wsh)}")
+    _inner(wsh, wst, "linear_i8: weight")
+    if orows != rows:
+        raise ValueError(f"linear_i8: out has {orows} rows, x has {rows}")
+    _dense(ssh, sst, (n,), "linear_i8: weight_scale")
+    devs = [d0, d1, d2, d3]
+    p_xs = p_b = None
+    if x_scale is not None:
+        p_xs, sh, st, t, d = _view(x_scale, "linear_i8: x_scale")
+        _type(t, "linear_i8: x_scale", ("float32",))
+        _dense(sh, st, (rows,) if len(sh) == 1 else xsh[:-1], "linear_i8: x_scale")
+        devs.append(d)
+    if bias is not None:
+        p_b, sh, st, t, d = _view(bias, "linear_i8: bias")
+        _type(t, "linear_i8: bias", ("float32",))
+        _dense(sh, st, (n,), "linear_i8: bias")
+        devs.append(d)
+    lib = _lib()
+    _check(lib, lib.tg_linear_i8(_device(*devs), stream, xp, xtype, rows, k, xs, wp, n, wst[0], sp, p_xs, p_b, bool(relu), op, otype, os_),
+           "tg_linear_i8")
+    return out
+
+
+def quantize_i8(x, q, scale, *, stream=0):
+    """q[..., k] = round(x[..., k] / scale[...]) (half to even), scale = max(max_k |x| / 127, 2^-126)
+
+    x float32 / float16 / bfloat16 [..., K], q int8 [..., K], scale float32 [rows].  q * scale is x to half a step.  A row with a
+    NaN or an infinity gets scale NaN and q 0: what is computed from it is NaN, not a plausible number.  Returns (q, scale)."""
+    xp, xsh, xst, xt, d0 = _view(x, "quantize_i8: x")
+    qp, qsh, qst, qt, d1 = _view(q, "quantize_i8: q")
+    sp, ssh, sst, stt, d2 = _view(scale, "quantize_i8: scale")
+    xtype = _type(xt, "quantize_i8: x", _FLOATS)
+    _type(qt, "quantize_i8: q", ("int8",))
+    _type(stt, "quantize_i8: scale", ("float32",))
+    rows, k, xs = _rows(xsh, xst, "quantize_i8: x")
+    if tuple(qsh) != tuple(xsh) and _rows(qsh, qst, "quantize_i8: q")[:2] != (rows, k):
+        raise ValueError(f"quantize_i8: q must have x's shape {tuple(xsh)}, got {tuple(qsh)}")
+    _, _, qs = _rows(qsh, qst, "quantize_i8: q")
+    _dense(ssh, sst, (rows,) if len(ssh) == 1 else xsh[:-1], "quantize_i8: scale")
+    lib = _lib()
+    _check(lib, lib.tg_quantize_i8(_device(d0, d1, d2), stream, xp, xtype, rows, k, xs, qp, qs, sp), "tg_quantize_i8")
+    return q, scale
+
+
+def beam_select_workspace(groups, beams_in, vocab, beams_out):
+    """Bytes of device memory beam_select needs as `workspace` for these sizes (0: none)."""
+    lib = _lib()
+    n = lib.tg_beam_select_workspace(groups, beams_in, vocab, beams_out)
+    if n < 0:
+        _check(lib, N.EINVAL, "tg_beam_select_workspace")
+    return n
+
+
+def beam_select(logits, scores, out_scores, parents, tokens, *, mask=None, finished=None, pad=0, normalize=True, workspace=None, stream=0):
+    """One step of a beam search for G independent groups of K beams over V entries.
+
+    Beam k of group g offers entry v at scores[g, k] + logits[g, k, v] - L, with L = log sum exp of the beam's allowed logits
+    (`normalize`) or 0 (logits are values that add up as they are).  mask uint8 / bool [G, K, V] (nonzero = allowed; broadcast axes may
+    have stride 0); a beam whose `finished` byte [G, K] is set offers only itself, as entry `pad` at its score.  A candidate
+    at -inf or NaN does not exist, so a beam of score -inf is dead and a row without allowed entries offers nothing.
+    out_scores float32, parents int32, tokens int32 [G, B] receive the B best, best first; equal ones in the order of
+    (beam, entry).  Missing ones: -inf, -1, -1.  logits float32 / float16 / bfloat16 [G, K, V].  `workspace`: uint8 memory of
+    beam_select_workspace(G, K, V, B) bytes, not shared with a call that may run at the same time.
+    Returns (out_scores, parents, tokens)."""
+    lp, lsh, lst, lt, d0 = _view(logits, "beam_select: logits")
+    sp, ssh, sst, stt, d1 = _view(scores, "beam_select: scores")
+    op, osh, ost, ot, d2 = _view(out_scores, "beam_select: out_scores")
+    pp, psh, pst, pt, d3 = _view(parents, "beam_select: parents")
+    tp, tsh, tst, tt, d4 = _view(tokens, "beam_select: tokens")
+    ltype = _type(lt, "beam_select: logits", _FLOATS)
+    _type(stt, "beam_select: scores", ("float32",))
+    _type(ot, "beam_select: out_scores", ("float32",))
+    _type(pt, "beam_select: parents", ("int32",))
+    _type(tt, "beam_select: tokens", ("int32",))
+    if len(lsh) != 3 or len(osh) != 2:
+        raise ValueError(f"beam_select: logits must be [G, K, V] and out_scores [G, B], got {tuple(lsh)} and {tuple(osh)}")
+    g, k, v = lsh
+    b = osh[1]
+    if not (1 <= k <= MAX_BEAMS and 1 <= b <= MAX_BEAMS and v >= 1):
+        raise ValueError(f"beam_select: {k} beams in, {b} out, {v} entries: 1 .. {MAX_BEAMS} beams and at least one entry are supported")
+    _inner(lsh, lst, "beam_select: logits")
+    _dense(ssh, sst, (g, k), "beam_select: scores")
+    for sh, st, what in ((osh, ost, "out_scores"), (psh, pst, "parents"), (tsh, tst, "tokens")):
+        _dense(sh, st, (g, b), "beam_select: " + what)
+    devs = [d0, d1, d2, d3, d4]
+    mp = fp = wp = None
+    mst = (0, 0)
+    if mask is not None:
+        mp, sh, mst, t, d = _view(mask, "beam_select: mask")
+        _type(t, "beam_select: mask", ("uint8", "bool"))
+        if tuple(sh) != (g, k, v):
+            raise ValueError(f"beam_select: mask must have shape {(g, k, v)}, got {tuple(sh)}")
+        _inner(sh, mst, "beam_select: mask")
+        devs.append(d)
+    if finished is not None:
+        fp, sh, st, t, d = _view(finished, "beam_select: finished")
+        _type(t, "beam_select: finished", ("uint8", "bool"))
+        _dense(sh, st, (g, k), "beam_select: finished")
+        devs.append(d)
+    nws = 0
+    if workspace is not None:
+        wp, sh, st, t, d = _view(workspace, "beam_select: workspace")
+        _type(t, "beam_select: workspace", ("uint8",))
+        if len(sh) != 1:
+            raise ValueError("beam_select: workspace must have one axis")
+        _dense(sh, st, sh, "beam_select: workspace")
+        nws = sh[0]
+        devs.append(d)
+    lib = _lib()
+    _check(lib, lib.tg_beam_select(_device(*devs), stream, lp, ltype, g, k, v, lst[0], lst[1], sp, mp, mst[0], mst[1], fp, pad, bool(normalize), b,
+                                   op, pp, tp, wp, nws), "tg_beam_select")
+    return out_scores, parents, tokens
+
+
+def _state(a, rows, what):
+    """(pointer, bytes of a row, stride of a row in bytes, device) of [G * K, ...] or [G, K, ...]"""
+    p, sh, st, t, d = _view(a, what)
+    if t not in _SIZES:
+        raise ValueError(f"{what}: unsupported element type {t}")
+    lead, n = 0, 1
+    while lead < len(sh) and (lead == 0 or n != rows):
+        n *= sh[lead]
+        lead += 1
+    if n != rows or lead == 0:
+        raise ValueError(f"{what}: the leading axes of {tuple(sh)} do not hold {rows} rows")
+    size, cols = _SIZES[t], 1
+    for s, k in zip(reversed(st[lead:]), reversed(sh[lead:])):
+        if k > 1 and s != cols:
+            raise ValueError(f"{what}: a row must be contiguous")
+        cols *= k
+    flat = _rows(tuple(sh[:lead]) + (1,), tuple(st[:lead]) + (1,), what)
+    stride = flat[2] if flat[0] > 1 else cols
+    return p, cols * size, stride * size, d
+
+
+def beam_reorder(states, parents, *, out=None, beams_in=None, stream=0):
+    """Rows that follow their beams: out[i][g, j] = states[i][g, parents[g, j]] for up to 24 arrays in one launch.
+
+    states: an array or a list of arrays [G * K, ...] or [G, K, ...] of any element type; parents int32 [G, B] as beam_select leaves
+    them.  K = beams_in, by default B.  out: the same number of arrays with B rows per group (not overlapping states), or None to
+    reorder in place (B = K).
+    A parent outside 0 .. K - 1 (the -1 of a missing beam) leaves its row as it was.  Returns out (or states)."""
+    single = not isinstance(states, (list, tuple))
+    src = [states] if single else list(states)
+    if out is None:
+        dst = src
+    else:
+        dst = list(out) if isinstance(out, (list, tuple)) else [out]
+        if len(dst) != len(src):
+            raise ValueError(f"beam_reorder: {len(src)} states, {len(dst)} outputs")
+    if len(src) > MAX_STATES:
+        raise ValueError(f"beam_reorder: {len(src)} arrays: up to {MAX_STATES} go into one call")
+    pp, psh, pst, pt, dev = _view(parents, "beam_reorder: parents")
+    _type(pt, "beam_reorder: parents", ("int32",))
+    if len(psh) != 2:
+        raise ValueError(f"beam_reorder: parents must be [G, B], got {tuple(psh)}")
+    _dense(psh, pst, psh, "beam_reorder: parents")
+    g, b = psh
+    n = len(src)
+    if n == 0 or g == 0:
+        return states if out is None else out
+    k = b if beams_in is None else int(beams_in)
+    if not (1 <= k <= MAX_BEAMS and 1 <= b <= MAX_BEAMS):
+        raise ValueError(f"beam_reorder: {k} beams in, {b} out: 1 .. {MAX_BEAMS} are supported")
+    if out is None and k != b:
+        raise ValueError(f"beam_reorder: in place takes as many beams out ({b}) as in ({k})")
+    arr = C.c_void_p * n
+    num = C.c_int64 * n
+    sv = [_state(a, g * k, f"beam_reorder: states[{i}]") for i, a in enumerate(src)]
+    dv = sv if out is None else [_state(a, g * b, f"beam_reorder: out[{i}]") for i, a in enumerate(dst)]
+    for i, (s, d) in enumerate(zip(sv, dv)):
+        if s[1] != d[1]:
+            raise ValueError(f"beam_reorder: rows of states[{i}] hold {s[1]} bytes, of out[{i}] {d[1]}")
+    lib = _lib()
+    _check(lib, lib.tg_beam_reorder(_device(dev, *(s[3] for s in sv), *(d[3] for d in dv)), stream, n, arr(*(s[0] for s in sv)),
+                                    arr(*(d[0] for d in dv)), num(*(s[1] for s in sv)), num(*(s[2] for s in sv)), num(*(d[2] for d in dv)),
+                                    g, k, b, pp), "tg_beam_reorder")
+    return states if out is None else out
