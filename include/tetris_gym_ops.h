@@ -29,12 +29,13 @@ extern "C" {
 
 #define TG_OPS_MAX_K 65536      /* longest sum of tg_linear_i8 (255 * 128 * 65536 < 2^31) */
 #define TG_OPS_MAX_BEAMS 64     /* beams of a group, in and out */
+#define TG_OPS_MAX_VOCAB (1 << 20) /* entries of tg_beam_select */
 #define TG_OPS_MAX_STATES 24    /* arrays of one tg_beam_reorder */
 
 const char* tg_ops_last_error(void);
 
 /* out[m][n] = act((sum_k x[m][k] * w[n][k]) * (x_scale[m] * w_scale[n]) + bias[n]): the sum in 32-bit integers (exact), the rest in
- * float32, one rounding to the output's type.  x: u8 or i8 [rows][k] (x_stride; any alignment: observations of 13 or 200 bytes),
+ * float32, one rounding to the output's type.  x: u8 or i8 [rows][k] (x_stride; any alignment: observations of 13 or 200 bytes; row strides up to 2^24),
  * w: i8 [n][k], w_scale f32[n], x_scale f32[rows] or NULL (1), bias f32[n] or NULL, relu: act = max(., 0), else identity.
  * out: f32 / f16 / bf16 [rows][n] (out_stride).  rows or n = 0 does nothing; k = 0 gives act(bias).  out must not overlap an input. */
 int tg_linear_i8(int device, void* stream, const void* x, int x_type, int64_t rows, int64_t k, int64_t x_stride, const int8_t* w, int64_t n,
@@ -55,7 +56,7 @@ int tg_quantize_i8(int device, void* stream, const void* x, int x_type, int64_t 
  * beams_in - 1), tokens i32 (0 .. vocab - 1); equal ones by beam, then by entry; within one beam entries rank by their logit.  Where
  * there are fewer: score -inf, parent -1, token -1.  logits: f32 / f16 / bf16 [groups][beams_in][vocab] (strides lg, lk; lk = 0 or
  * lg = 0 broadcasts), mask likewise (mg, mk), scores / finished [groups][beams_in] and the outputs [groups][beams_out] contiguous.
- * c is held in 64 bits, L to about 1e-14 of its value.  workspace: tg_beam_select_workspace bytes (0 for small searches), 16-byte
+ * c is held in 64 bits, L to 1e-12.  workspace: tg_beam_select_workspace bytes (0 for small searches), 16-byte
  * aligned, not shared by calls that may run at the same time. */
 int64_t tg_beam_select_workspace(int64_t groups, int64_t beams_in, int64_t vocab, int64_t beams_out);
 int tg_beam_select(int device, void* stream, const void* logits, int type, int64_t groups, int64_t beams_in, int64_t vocab, int64_t lg,
@@ -73,8 +74,17 @@ int tg_beam_reorder(int device, void* stream, int n, const void* const* src, voi
 
 /* The same for an engine: env g * beams + j becomes a copy of env g * beams + parents[g][j] in every respect (board, record, generator,
  * observation, last outputs, episode statistics), in place, asynchronous on the handle's stream.  batch must be a multiple of beams
- * and every env must have been reset. */
+ * and every env must have been reset (NUMPY rules). */
 int tg_reorder_beams(tg_handle* h, const int32_t* parents, int beams);
+
+/* The bookkeeping of a search between tg_beam_select and a transition, for groups * beams environments: gain_out = gain_in of the parent
+ * and actions = the token where a beam has a parent; gain_out = -inf (a dead beam) and action 0 where it has none.  gain_out must not
+ * overlap gain_in. */
+int tg_beam_advance(int device, void* stream, int64_t groups, int64_t beams, const int32_t* parents, const int32_t* tokens,
+                    const float* gain_in, float* gain_out, int32_t* actions);
+
+/* ... and behind the transition: gain += reward, or -inf where the game has ended (n environments). */
+int tg_beam_collect(int device, void* stream, int64_t n, const tg_step_out* out, float* gain);
 
 /* The handle's stream (a hipStream_t), for calls above that shall run in order with the handle's own. */
 int tg_stream(tg_handle* h, void** stream);

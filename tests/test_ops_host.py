@@ -161,3 +161,21 @@ def test_null_pointers_and_types_are_refused_by_the_c_entries():
     assert lib.tg_beam_reorder(0, None, 1, (C.c_void_p * 1)(None), (C.c_void_p * 1)(None), one, one, one, 1, 1, 1, C.c_void_p(64)) == N.EINVAL
     assert lib.tg_reorder_beams(None, None, 1) == N.EINVAL and lib.tg_stream(None, None) == N.EINVAL
     assert lib.tg_linear_i8(0, None, None, N.T_U8, 0, 1, 1, None, 1, 1, None, None, None, 0, None, N.T_F32, 1) == N.OK  # nothing to do
+
+
+def test_scorer_refusals():
+    import numpy as np
+
+    from tetris_gymnasium_amd import PlacementScorer
+
+    w, s = np.ones((1, 13), np.int8), np.ones(1, np.float32)
+    assert PlacementScorer([(w, s, None)]).n_features == 13
+    for layers in ([], [(w.astype(np.float32), s, None)], [(w, np.ones(2), None)], [(w, s, np.ones(2))], [(np.ones((3, 13), np.int8), np.ones(3), None)],
+                   [(np.ones((3, 13), np.int8), np.ones(3), None), (np.ones((1, 4), np.int8), s, None)]):
+        with pytest.raises(ValueError):
+            PlacementScorer(layers)
+    with pytest.raises(ValueError, match="finite"):
+        PlacementScorer.from_float([(np.full((1, 13), np.nan), None)])
+    f = np.array([[1.0, -2.0, 0.25]], np.float32)
+    (q, sc, _), = PlacementScorer.from_float([(f, None)]).layers
+    assert q.tolist() == [[64, -127, 16]] and sc[0] == np.float32(2.0) / np.float32(127)  # 63.5 to even, 15.875

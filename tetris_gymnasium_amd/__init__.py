@@ -5,5 +5,6 @@ Python host code calls hand-written HIP (gfx950) through a thin ctypes C ABI.  N
 from . import _native  # noqa: F401
 from .engine import DeviceArray, Engine, EngineError  # noqa: F401
 from . import ops  # noqa: F401
+from .search import BeamSearch, PlacementScorer  # noqa: F401
 
-__all__ = ["DeviceArray", "Engine", "EngineError", "ops"]
+__all__ = ["BeamSearch", "DeviceArray", "Engine", "EngineError", "PlacementScorer", "ops"]

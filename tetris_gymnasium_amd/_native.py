@@ -119,6 +119,8 @@ OPS_SYMBOLS = {
     "tg_beam_select_workspace": (_i64, [_i64] * 4),
     "tg_beam_select": (_i, [_i, _vp, _vp, _i] + [_i64] * 5 + [_vp, _vp, _i64, _i64, _vp, _i, _i, _i64, _vp, _vp, _vp, _vp, _i64]),
     "tg_beam_reorder": (_i, [_i, _vp, _i, _pp, _pp, C.POINTER(_i64), C.POINTER(_i64), C.POINTER(_i64), _i64, _i64, _i64, _vp]),
+    "tg_beam_advance": (_i, [_i, _vp, _i64, _i64] + [_vp] * 5),
+    "tg_beam_collect": (_i, [_i, _vp, _i64, _vp, _vp]),
     "tg_reorder_beams": (_i, [_vp, _vp, _i]),
     "tg_stream": (_i, [_vp, _pp]),
 }

@@ -2198,7 +2198,8 @@ int tg_reorder_beams(tg_handle* h, const int32_t* parents, int beams) {
   if (!parents) return fail(h, TG_EINVAL, "tg_reorder_beams: null parents");
   if (beams < 1 || beams > TG_OPS_MAX_BEAMS || h->B % beams)
     return fail(h, TG_EINVAL, "tg_reorder_beams: %d beams: 1 .. %d that divide the batch of %d are supported", beams, TG_OPS_MAX_BEAMS, h->B);
-  if (const void* z = std::memchr(h->rng_valid.data(), 0, (size_t)h->B))
+  const void* z = h->cfg.ruleset == TG_RULESET_NUMPY ? std::memchr(h->rng_valid.data(), 0, (size_t)h->B) : nullptr;
+  if (z)  // (a later tg_reset without seeds would seed such an env by its index: host state that cannot follow a parent known to the device only)
     return fail(h, TG_EINVAL, "tg_reorder_beams: env %d was never reset", (int)((const uint8_t*)z - h->rng_valid.data()));
   HIPCHK(h, hipSetDevice(h->cfg.device));
   { int rcj = join_shards(h); if (rcj != TG_OK) return rcj; }

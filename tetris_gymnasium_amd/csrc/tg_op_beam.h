@@ -1,5 +1,6 @@
 // tg_beam_select, tg_beam_reorder: one step of a beam search over beams and entries, and the rows that follow their beams.
 #pragma once
+#include "../../include/tetris_gym_hip.h"
 #include "tg_op_common.h"
 
 namespace tg {
@@ -18,93 +19,364 @@ struct SelectArgs {
   int k, v, beams, pad, norm;
 };
 
-// a candidate in the order of the result: better() is a strict total order (within a beam the score never falls with the logit)
-struct Cand { double s; float x; int row, v; };
-__device__ __forceinline__ bool better(const Cand& a, const Cand& b) {
-  if (a.row == b.row) return a.x > b.x || (a.x == b.x && a.v < b.v);
-  return a.s > b.s || (a.s == b.s && a.row < b.row);
+// e^d for d <= 0 to 3e-13 of its value (NaN stays, far below zero gives 0): 2^n e^r with |r| <= ln(2)/2 and the exponential series to
+// r^10 (the next term is below 0.3466^11 / 11! = 2.2e-13).  n comes out of the low bits of d log2(e) + 1.5 * 2^52.
+__device__ __forceinline__ double exp_neg(double d) {
+  d = d < -800.0 ? -800.0 : d;
+  const double big = 6755399441055744.0, z = fma(d, 1.4426950408889634, big), n = z - big;
+  double r = fma(-n, 0x1.62e42fefa0000p-1, d);  // ln 2 in two parts; n times the first (41 bits) is exact
+  r = fma(-n, 0x1.cf79abc9e3b3ap-41, r);
+  double p = 1.0 / 3628800;
+  p = fma(p, r, 1.0 / 362880);
+  p = fma(p, r, 1.0 / 40320);
+  p = fma(p, r, 1.0 / 5040);
+  p = fma(p, r, 1.0 / 720);
+  p = fma(p, r, 1.0 / 120);
+  p = fma(p, r, 1.0 / 24);
+  p = fma(p, r, 1.0 / 6);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return ldexp(p, (int)(uint32_t)(uint64_t)__double_as_longlong(z));
 }
-__device__ __forceinline__ Cand cand_none() { return {-__builtin_inf(), -__builtin_inff(), 1 << 30, 1 << 30}; }
 
-// One workgroup per group: the rows' log-sums, then one scan per result for the best candidate behind the last one.
-template <class T> __global__ __launch_bounds__(256) void select_scan_kernel(const SelectArgs a) {
-  __shared__ double lse[64], red[4];
-  __shared__ float redf[4];
-  __shared__ Cand best[4];
-  const int64_t g = blockIdx.x;
-  const int t = threadIdx.x, wave = t >> 6;
-  const T* x = (const T*)a.x + g * a.lg;
-  const uint8_t* mask = a.mask ? a.mask + g * a.mg : nullptr;
-  auto at = [&](int j, int i) {  // the logit of an allowed entry; what is not allowed reads as -inf
-    if (mask && !mask[j * a.mk + i]) return -__builtin_inff();
-    return to_f32(x[j * a.lk + i]);
-  };
-  for (int j = 0; j < a.k; ++j) {
+// A candidate as two words, larger = better, {0, .} = none: the score, then (beam, logit, entry) — within a beam the score never falls
+// with the logit, so entries of one beam rank by their logit, and by their place where that is equal.
+struct Key { uint64_t s, r; };
+__device__ __forceinline__ bool better(const Key& a, const Key& b) { return a.s > b.s || (a.s == b.s && a.r > b.r); }
+__device__ __forceinline__ uint64_t key_rest(int row, uint32_t xo, int v) {
+  return ((uint64_t)(63 - row) << 56) | ((uint64_t)xo << 24) | (uint64_t)(0xFFFFFF - v);
+}
+__device__ __forceinline__ Key make_key(double c, int row, uint32_t xo, int v) {
+  Key k;
+  k.s = c > -__builtin_inf() ? order_f64(c) : 0;  // (NaN and -inf are no candidates)
+  k.r = key_rest(row, xo, v);
+  return k;
+}
+__device__ __forceinline__ void put_result(const SelectArgs& a, int64_t o, const Key& k) {
+  const bool none = k.s == 0;
+  a.out_scores[o] = none ? -__builtin_inff() : (float)unorder_f64(k.s);
+  a.parents[o] = none ? -1 : 63 - (int)(k.r >> 56);
+  a.tokens[o] = none ? -1 : 0xFFFFFF - (int)(k.r & 0xFFFFFF);
+}
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int l) {  // the value of lane l (uniform), in scalar registers
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l) | ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l) << 32);
+}
+__device__ __forceinline__ uint64_t max_u64(uint64_t a, uint64_t b) { return a > b ? a : b; }
+
+// A bound that at least `beams` (or all) of the wave's lane maxima reach: with up to 16 beams the beams-th largest of the 16 maxima of
+// four lanes, else of the 64 lane maxima, by counting for each how many are larger.  Fewer than that: 1 (any candidate).
+__device__ __forceinline__ uint64_t wave_bound(uint64_t m, int beams) {
+  const bool quads = beams <= 16;
+  if (quads) m = group_reduce<4>(m, max_u64);
+  int larger = 0;
+  if (quads) {
+#pragma unroll
+    for (int l = 0; l < 64; l += 4) larger += lane_u64(m, l) > m;
+  } else {
+    for (int l = 0; l < 64; ++l) larger += lane_u64(m, l) > m;
+  }
+  // of the values with fewer than `beams` larger ones the smallest: equal values count once, so this is never above the beams-th
+  const uint64_t low = group_reduce<64>(larger < beams ? m : ~(uint64_t)0, [](uint64_t a, uint64_t b) { return a < b ? a : b; });
+  return low ? low : 1;
+}
+
+// Of N candidates per lane the best `beams` of the wave, handed to put(rank, key) in descending order; returns how many there are.
+// What reaches the bound is packed into one candidate per lane through LDS (64 keys per wave) and ranked by counting; where more than
+// 64 reach it (many equal ones, many beams), the best is taken out `beams` times instead.
+template <int N, class F> __device__ __forceinline__ int wave_top(Key (&k)[N], int beams, Key* lds, F put) {
+  const int lane = threadIdx.x & 63;
+  uint64_t m = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = max_u64(m, k[i].s);
+  const uint64_t bound = wave_bound(m, beams);
+  int n = 0, at[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint64_t b = __ballot(k[i].s >= bound);
+    at[i] = n + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+    n += (int)__popcll(b);
+  }
+  if (n <= 64) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (k[i].s >= bound) lds[at[i]] = k[i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    Key c = {0, 0};
+    if (lane < n) c = lds[lane];
+    int rank = 0;
+    for (int l = 0; l < n; ++l) {
+      const Key o = {lane_u64(c.s, l), lane_u64(c.r, l)};
+      rank += better(o, c);
+    }
+    if (lane < n && rank < beams) put(rank, c);
+    __builtin_amdgcn_wave_barrier();
+    return n < beams ? n : beams;
+  }
+  for (int b = 0; b < beams; ++b) {
+    Key c = {0, 0};
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (better(k[i], c)) c = k[i];
+    const uint64_t s = group_reduce<64>(c.s, max_u64), r = group_reduce<64>(c.s == s ? c.r : (uint64_t)0, max_u64);
+    if (s == 0) return b;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (k[i].s == s && k[i].r == r) {
+        put(b, k[i]);
+        k[i].s = 0;
+      }
+  }
+  return beams;
+}
+
+// Small searches: a wave per group, L = the power of two below 64 / K lanes per beam, N entries per lane (V <= L * N).  The log-sum of
+// a beam is a reduction over its L lanes.  Everything stays in registers; the input is read once.
+template <class T, int N> __global__ __launch_bounds__(256) void select_small_kernel(const SelectArgs a, int shift) {
+  __shared__ Key lds[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t g = (int64_t)blockIdx.x * 4 + wave;
+  if (g >= a.groups) return;
+  const int L = 1 << shift, j = lane >> shift, sub = lane & (L - 1);
+  const bool here = j < a.k;
+  const int jj = here ? j : 0;
+  const float sc = a.scores[g * a.k + jj];
+  const bool done = a.finished && a.finished[g * a.k + jj];
+  const T* x = (const T*)a.x + g * a.lg + jj * a.lk;
+  const uint8_t* mask = a.mask ? a.mask + g * a.mg + jj * a.mk : nullptr;
+  T raw[N];
+  uint8_t ok[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {  // (all loads first)
+    const int v = sub + i * L, vv = v < a.v ? v : 0;
+    raw[i] = x[vv];
+    ok[i] = mask ? mask[vv] : 1;
+  }
+  float e[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) e[i] = here && !done && ok[i] && sub + i * L < a.v ? to_f32(raw[i]) : -__builtin_inff();
+  double lse = 0;
+  if (a.norm) {
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, e[i]);
+    auto fm = [](float p, float q) { return fmaxf(p, q); };
+    if (L > 1) m = fm(m, xor_lane<1>(m));
+    if (L > 2) m = fm(m, xor_lane<2>(m));
+    if (L > 4) m = fm(m, xor_lane<4>(m));
+    if (L > 8) m = fm(m, xor_lane<8>(m));
+    if (L > 16) m = fm(m, xor_lane<16>(m));
+    if (L > 32) m = fm(m, xor_lane<32>(m));
+    double s = 0;
+    const double md = m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) s += exp_neg((double)e[i] - md);  // (m = -inf, +inf or a NaN among them: NaN, no candidate)
+    if (L > 1) s += xor_lane<1>(s);
+    if (L > 2) s += xor_lane<2>(s);
+    if (L > 4) s += xor_lane<4>(s);
+    if (L > 8) s += xor_lane<8>(s);
+    if (L > 16) s += xor_lane<16>(s);
+    if (L > 32) s += xor_lane<32>(s);
+    lse = md + log(s);
+  }
+  Key k[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const double c = e[i] > -__builtin_inff() ? (double)sc + ((double)e[i] - lse) : -__builtin_inf();
+    k[i] = make_key(c, jj, order_f32(e[i]), sub + i * L);
+  }
+  if (here && done && sub == 0) k[0] = make_key((double)sc, j, 0, a.pad);
+  const int64_t o = g * a.beams;
+  const int n = wave_top(k, a.beams, lds[wave], [&](int rank, const Key& c) { put_result(a, o + rank, c); });
+  if (lane >= n && lane < a.beams) put_result(a, o + lane, Key{0, 0});
+}
+
+// Large searches, first step: a workgroup per (beam, chunk of 256 * E entries), the chunk in registers: its maximum, its sum of
+// exponentials against that maximum, and its best `beams` entries by (logit, place).
+// Keys are unique, so `beams` quads of lanes (17 and more: lanes) of a wave reach its bound, with all their E entries at most.
+__device__ __host__ __forceinline__ int select_list(int beams, int e) {
+  const int lanes = 4 * beams * (beams <= 16 ? 4 : 1);
+  return (lanes < 256 ? lanes : 256) * e;
+}
+struct SelectPart { double s; float m; int n; };  // then uint64_t[beams]: order(logit) << 32 | ~entry, descending, n of them
+__device__ __host__ __forceinline__ int64_t select_part_bytes(int beams) { return 16 + 8 * (int64_t)beams; }
+
+template <class T, int E> __global__ __launch_bounds__(256) void select_chunk_kernel(const SelectArgs a, int chunks, uint8_t* ws) {
+  constexpr int V = 16 / (int)sizeof(T), NV = E / V;
+  extern __shared__ uint64_t list[];  // select_list(beams, E): what reaches its wave's bound
+  __shared__ float wm[4];
+  __shared__ double wsum[4];
+  __shared__ int count;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int64_t row = blockIdx.x / chunks, g = row / a.k;
+  const int chunk = blockIdx.x % chunks, j = (int)(row % a.k);
+  uint8_t* part = ws + (int64_t)blockIdx.x * select_part_bytes(a.beams);
+  SelectPart* head = (SelectPart*)part;
+  uint64_t* keys = (uint64_t*)(part + 16);
+  if ((a.finished && a.finished[row]) || !(a.scores[row] > -__builtin_inff())) {  // (offers nothing of its own)
+    if (t == 0) *head = {0.0, -__builtin_inff(), 0};
+    return;
+  }
+  if (t == 0) count = 0;
+  const T* x = (const T*)a.x + g * a.lg + j * a.lk;
+  const uint8_t* mask = a.mask ? a.mask + g * a.mg + j * a.mk : nullptr;
+  const int v0 = chunk * (256 * E) + t * V;
+  float e[E];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = v0 + i * 256 * V;
+    if (v + V <= a.v) {
+      const v4i u = load16(x + v);
+      T h[V];
+      __builtin_memcpy(h, &u, 16);
+      uint8_t ok[V];
+      if (mask) __builtin_memcpy(ok, mask + v, V);
+#pragma unroll
+      for (int q = 0; q < V; ++q) e[i * V + q] = !mask || ok[q] ? to_f32(h[q]) : -__builtin_inff();
+    } else {
+#pragma unroll
+      for (int q = 0; q < V; ++q) e[i * V + q] = v + q < a.v && (!mask || mask[v + q]) ? to_f32(x[v + q]) : -__builtin_inff();
+    }
+  }
+  float m = -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < E; ++i) m = fmaxf(m, e[i]);
+  const float lm = m;  // (of the lane; a NaN is not in it)
+  m = group_reduce<64>(m, [](float p, float q) { return fmaxf(p, q); });
+  if (lane == 0) wm[wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+  double s = 0;
+  if (a.norm) {
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < E; ++i) nan |= e[i] != e[i];
+    const double md = m > -__builtin_inff() ? (double)m : 0.0;  // (nothing allowed: a sum of 0)
+#pragma unroll
+    for (int i = 0; i < E; ++i) s += exp_neg((double)e[i] - md);
+    if (nan || m == __builtin_inff()) s = __builtin_nan("");
+    s = group_reduce<64>(s, [](double p, double q) { return p + q; });
+    if (lane == 0) wsum[wave] = s;
+  }
+  // the lane's best entry, the wave's bound, and what reaches it
+  int best = 0;
+  float bx = -__builtin_inff();
+#pragma unroll
+  for (int i = E - 1; i >= 0; --i)
+    if (e[i] == lm && lm > -__builtin_inff()) { best = i; bx = lm; }
+  auto entry = [&](int i) { return v0 + (i / V) * 256 * V + i % V; };
+  auto key = [&](float f, int v) { return f > -__builtin_inff() ? ((uint64_t)order_f32(f) << 32) | (uint32_t)~v : 0ull; };
+  const uint64_t bound = wave_bound(key(bx, entry(best)), a.beams);
+  const uint32_t bhi = (uint32_t)(bound >> 32);
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const bool maybe = e[i] > -__builtin_inff() && order_f32(e[i]) >= bhi;
+    if (__ballot(maybe)) {
+      const uint64_t k = maybe ? key(e[i], entry(i)) : 0;
+      if (k >= bound) list[atomicAdd(&count, 1)] = k;
+    }
+  }
+  __syncthreads();
+  const int n = count, keep = n < a.beams ? n : a.beams;
+  for (int i = t; i < n; i += 256) {
+    const uint64_t k = list[i];
+    int rank = 0;
+    for (int l = 0; l < n; ++l) rank += list[l] > k;
+    if (rank < keep) keys[rank] = k;
+  }
+  if (t == 0) *head = {a.norm ? wsum[0] + wsum[1] + wsum[2] + wsum[3] : 0.0, m, keep};
+}
+
+// ... second step: a wave per group puts the chunks' sums and lists together.  Candidates come in rounds of 64 * 4, the first entries of
+// all lists before the second ones, so that later rounds soon hold nothing better than the `beams` already found.
+__global__ __launch_bounds__(64) void select_merge_kernel(const SelectArgs a, int chunks, const uint8_t* ws) {
+  constexpr int N = 4;
+  __shared__ Key lds[64], top[64];
+  __shared__ double lse[64];
+  const int lane = threadIdx.x;
+  const int64_t g = blockIdx.x, pb = select_part_bytes(a.beams);
+  const uint8_t* base = ws + g * a.k * chunks * pb;
+  if (lane < a.k) {
     double L = 0;
     if (a.norm) {
       float m = -__builtin_inff();
-      bool nan = false;
-      for (int i = t; i < a.v; i += 256) {
-        const float e = at(j, i);
-        nan |= e != e;
-        m = fmaxf(m, e);
+      for (int c = 0; c < chunks; ++c) m = fmaxf(m, ((const SelectPart*)(base + ((int64_t)lane * chunks + c) * pb))->m);
+      double s = 0;
+      for (int c = 0; c < chunks; ++c) {
+        const SelectPart* h = (const SelectPart*)(base + ((int64_t)lane * chunks + c) * pb);
+        const double hs = h->s;
+        if (hs != 0.0) s += hs * exp_neg((double)h->m - (double)m);
       }
-      m = group_reduce<64>(m, [](float p, float q) { return fmaxf(p, q); });
-      if ((t & 63) == 0) redf[wave] = m;
-      __syncthreads();
-      m = fmaxf(fmaxf(redf[0], redf[1]), fmaxf(redf[2], redf[3]));
-      double s = nan ? __builtin_nan("") : 0.0;
-      if (m > -__builtin_inff())
-        for (int i = t; i < a.v; i += 256) s += exp((double)at(j, i) - (double)m);  // (m = +inf: NaN)
-      s = group_reduce<64>(s, [](double p, double q) { return p + q; });
-      if ((t & 63) == 0) red[wave] = s;
-      __syncthreads();
-      s = red[0] + red[1] + red[2] + red[3];
       L = (double)m + log(s);
-      __syncthreads();
     }
-    if (t == 0) lse[j] = L;
+    lse[lane] = L;
   }
+  int found = 0;
   __syncthreads();
-  Cand last = {__builtin_inf(), __builtin_inff(), -1, -1};
-  for (int b = 0; b < a.beams; ++b) {
-    Cand mine = cand_none();
-    for (int j = 0; j < a.k; ++j) {
-      const float sc = a.scores[g * a.k + j];
-      if (a.finished && a.finished[g * a.k + j]) {
-        const Cand c = {(double)sc, 0.0f, j, a.pad};
-        if (t == 0 && c.s > -__builtin_inf() && better(last, c) && better(c, mine)) mine = c;
-        continue;
+  const int lists = a.k * chunks;
+  const int64_t total = (int64_t)lists * a.beams;
+  Key bottom = {0, 0};  // the worst of the `beams` found so far, or none
+  for (int64_t i0 = -64; i0 < total;) {
+    Key k[N];
+    bool any = false;
+    if (i0 < 0) {  // first the finished beams, a candidate each
+#pragma unroll
+      for (int i = 0; i < N; ++i) k[i] = {0, 0};
+      if (lane < a.k && a.finished && a.finished[g * a.k + lane]) {
+        k[0] = make_key((double)a.scores[g * a.k + lane], lane, 0, a.pad);
+        any = k[0].s != 0;
       }
-      for (int i = t; i < a.v; i += 256) {
-        const float e = at(j, i);
-        const Cand c = {(double)sc + ((double)e - lse[j]), e, j, i};
-        if (c.s > -__builtin_inf() && e > -__builtin_inff() && better(last, c) && better(c, mine)) mine = c;
+      i0 = 0;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int64_t c = i0 + i * 64 + lane;
+        k[i] = {0, 0};
+        if (c < total) {
+          const int rank = (int)(c / lists), l = (int)(c - (int64_t)rank * lists), row = l / chunks;
+          const uint8_t* part = base + (int64_t)l * pb;
+          if (rank < ((const SelectPart*)part)->n) {
+            const uint64_t u = ((const uint64_t*)(part + 16))[rank];
+            const float x = unorder_f32((uint32_t)(u >> 32));
+            k[i] = make_key((double)a.scores[g * a.k + row] + ((double)x - lse[row]), row, (uint32_t)(u >> 32), (int)~(uint32_t)u);
+            if (!better(k[i], bottom)) k[i].s = 0;
+            any |= k[i].s != 0;
+          }
+        }
       }
+      i0 += 64 * N;
     }
-    auto pick = [](Cand p, const Cand& q) { return better(q, p) ? q : p; };
-    for (int d = 32; d; d >>= 1) {
-      Cand o;
-      o.s = __shfl_xor(mine.s, d);
-      o.x = __shfl_xor(mine.x, d);
-      o.row = __shfl_xor(mine.row, d);
-      o.v = __shfl_xor(mine.v, d);
-      mine = pick(mine, o);
-    }
-    if ((t & 63) == 0) best[wave] = mine;
-    __syncthreads();
-    mine = pick(pick(pick(best[0], best[1]), best[2]), best[3]);
-    __syncthreads();
-    last = mine;
-    const bool none = mine.row == 1 << 30;
-    if (t == 0) {
-      const int64_t o = g * a.beams + b;
-      a.out_scores[o] = none ? -__builtin_inff() : (float)mine.s;
-      a.parents[o] = none ? -1 : mine.row;
-      a.tokens[o] = none ? -1 : mine.v;
-    }
-    if (none) last = cand_none();  // (nothing is behind it)
+    if (!__ballot(any)) continue;
+    Key all[N + 1];
+#pragma unroll
+    for (int i = 0; i < N; ++i) all[i] = k[i];
+    all[N] = lane < found ? top[lane] : Key{0, 0};
+    __builtin_amdgcn_wave_barrier();
+    found = wave_top(all, a.beams, lds, [&](int rank, const Key& c) { top[rank] = c; });
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (found == a.beams) bottom = top[a.beams - 1];
   }
+  if (lane < a.beams) put_result(a, g * a.beams + lane, lane < found ? top[lane] : Key{0, 0});
+}
+
+// which of them, by sizes alone (the workspace goes by it)
+struct SelectPlan { bool small; int shift, per_lane, e, chunks; };
+inline SelectPlan select_plan(int64_t groups, int64_t k, int64_t v) {
+  SelectPlan p{};
+  p.shift = 6;
+  while (k << p.shift > 64) --p.shift;
+  const int64_t per = (v + (1 << p.shift) - 1) >> p.shift;
+  if (per <= 16) {
+    p.small = true;
+    p.per_lane = (int)per;
+    return p;
+  }
+  p.e = v <= 2048 ? 8 : v <= 4096 ? 16 : 32;
+  while (p.e > 8 && groups * k * ((v + 256 * p.e - 1) / (256 * p.e)) < 1024) p.e /= 2;  // enough workgroups for four per compute unit
+  p.chunks = (int)((v + 256 * p.e - 1) / (256 * p.e));
+  return p;
 }
 
 // ---- reorder -------------------------------------------------------------------------------------------------------------------
@@ -169,6 +441,22 @@ __global__ __launch_bounds__(256) void reorder_kernel(const ReorderArgs p) {
     case 1: reorder_item<uint16_t>(a, p, item - a.first, lane); break;
     default: reorder_item<uint8_t>(a, p, item - a.first, lane); break;
   }
+}
+
+// ---- bookkeeping of a search around a transition: a thread per environment, bound by the launch --------------------------------------
+__global__ __launch_bounds__(256) void advance_kernel(const int32_t* parents, const int32_t* tokens, const float* gain_in, float* gain_out,
+                                                      int32_t* actions, int64_t n, int beams) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const int p = parents[i];
+  const bool ok = p >= 0 && p < beams;
+  gain_out[i] = ok ? gain_in[i / beams * beams + p] : -__builtin_inff();
+  actions[i] = ok ? tokens[i] : 0;
+}
+__global__ __launch_bounds__(256) void collect_kernel(const tg_step_out* out, float* gain, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  gain[i] = out[i].terminated ? -__builtin_inff() : gain[i] + out[i].reward;
 }
 
 }  // namespace ops

@@ -65,6 +65,56 @@ template <class F> int by_float(int t, F f) {
   return f(bf16_t{});
 }
 
+constexpr int kUnits = 256;  // compute units
+
+template <class OT, bool U8, int KS> void linear_rows(const LinearArgs& a, hipStream_t st) {
+  const int64_t cols = (a.n + 63) / 64;
+  const int strips = cols >= 4 ? 4 : cols == 2 ? 2 : 1, below = 4 / strips;
+  const int64_t gy = (cols + strips - 1) / strips, tiles = (a.rows + 15) / 16;
+  // as many workgroups as stay resident (two per unit for the widest variant), each with a run of tiles
+  int64_t gx = (kUnits * 4 + gy - 1) / gy;
+  if (gx > (tiles + below - 1) / below) gx = (tiles + below - 1) / below;
+  hipLaunchKernelGGL((linear_rows_kernel<OT, U8, KS>), dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, st, a, strips);
+}
+
+template <class OT, bool U8, int T, int U> void linear_few(const LinearArgs& a, hipStream_t st) {
+  int waves = (int)((a.k + 255) / 256);
+  waves = waves < 1 ? 1 : waves > 8 ? 8 : waves;
+  const int kw = (int)((a.k + waves * 64 - 1) / (waves * 64)) * 64;
+  hipLaunchKernelGGL((linear_few_kernel<OT, U8, T, U>), dim3((unsigned)((a.n + 16 * T - 1) / (16 * T)), (unsigned)((a.rows + 16 * U - 1) / (16 * U))),
+                     dim3(64 * waves), 0, st, a, kw);
+}
+
+template <class OT, bool U8, int BM, int BN, int WM, int WN, bool AL> void linear_tile(const LinearArgs& a, hipStream_t st) {
+  const int64_t mt = (a.rows + BM - 1) / BM, nt = (a.n + BN - 1) / BN;
+  const int64_t most = kMaxGrid / nt;  // row tiles of one launch
+  for (int64_t i = 0; i < mt; i += most) {
+    LinearArgs b = a;
+    b.x = a.x + i * BM * a.x_stride;
+    b.xs = a.xs ? a.xs + i * BM : nullptr;
+    b.out = (OT*)a.out + i * BM * a.out_stride;
+    b.rows = a.rows - i * BM < most * BM ? a.rows - i * BM : most * BM;
+    const int m = (int)((b.rows + BM - 1) / BM);
+    hipLaunchKernelGGL((linear_tile_kernel<OT, U8, BM, BN, WM, WN, AL>), dim3((unsigned)(m * nt)), dim3(WM * WN * 64), 2 * (BM + BN) * 128, st, b, m, (int)nt);
+  }
+}
+
+template <class OT, bool U8> void linear_launch(const LinearArgs& a, hipStream_t st) {
+  if (a.rows <= 64) {
+    if (a.rows <= 16) return linear_few<OT, U8, 1, 1>(a, st);
+    if (a.rows <= 32) return linear_few<OT, U8, 2, 2>(a, st);
+    return linear_few<OT, U8, 2, 4>(a, st);
+  }
+  if (a.k <= 64) return linear_rows<OT, U8, 1>(a, st);
+  if (a.k <= 128) return linear_rows<OT, U8, 2>(a, st);
+  if (a.k <= 256) return linear_rows<OT, U8, 4>(a, st);
+  const bool al = (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.x_stride | (uintptr_t)a.w_stride | (uintptr_t)a.k) & 15) == 0;
+  const int64_t big = ((a.rows + 255) / 256) * ((a.n + 255) / 256);
+  if (!al) return linear_tile<OT, U8, 128, 128, 2, 2, false>(a, st);
+  if (big >= kUnits) return linear_tile<OT, U8, 256, 256, 2, 4, true>(a, st);
+  return linear_tile<OT, U8, 128, 128, 2, 2, true>(a, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -82,7 +132,7 @@ int tg_linear_i8(int device, void* stream, const void* x, int x_type, int64_t ro
   if ((rows > 1 && (x_stride < 0 || x_stride > (1 << 24))) || (n > 1 && (w_stride < k || w_stride > (1 << 24))))
     return fail(TG_EINVAL, "tg_linear_i8: row strides (x %lld, w %lld) out of range", (long long)x_stride, (long long)w_stride);
   if (rows > 1 && (out_stride < n || out_stride > (1 << 24))) return fail(TG_EINVAL, "tg_linear_i8: the output's row stride %lld must be n .. 2^24", (long long)out_stride);
-  if (n > (1 << 24) || rows > ((int64_t)1 << 34)) return fail(TG_EINVAL, "tg_linear_i8: n = %lld or rows = %lld too large", (long long)n, (long long)rows);
+  if (n > (1 << 22) || rows > ((int64_t)1 << 34)) return fail(TG_EINVAL, "tg_linear_i8: n = %lld or rows = %lld too large", (long long)n, (long long)rows);
   if (!out || !w_scale || (k && (!x || !w))) return fail(TG_EINVAL, "tg_linear_i8: null pointer");
   const int os = type_size(out_type);
   if ((uintptr_t)out % os || (uintptr_t)w_scale % 4 || (uintptr_t)x_scale % 4 || (uintptr_t)bias % 4)
@@ -98,18 +148,8 @@ int tg_linear_i8(int device, void* stream, const void* x, int x_type, int64_t ro
                (uintptr_t)out % 16 == 0 && (out_stride * os) % 16 == 0};
   by_float(out_type, [&](auto o) {
     using OT = decltype(o);
-    // (grid.x holds rows: 2^34 / 64 workgroups; grid.y columns: 2^24 / 64 would pass 65 535, so wide outputs go in parts)
-    for (int64_t c = 0; c < n; c += 65535 * 64) {
-      LinearArgs b = a;
-      b.w = w + c * w_stride;
-      b.ws = w_scale + c;
-      b.bias = bias ? bias + c : nullptr;
-      b.out = (OT*)out + c;
-      b.n = n - c < 65535 * 64 ? n - c : 65535 * 64;
-      const dim3 grid((unsigned)((rows + 63) / 64), (unsigned)((b.n + 63) / 64));
-      if (x_type == kU8) hipLaunchKernelGGL((linear_wave_kernel<OT, true>), grid, dim3(256), 0, (hipStream_t)stream, b);
-      else hipLaunchKernelGGL((linear_wave_kernel<OT, false>), grid, dim3(256), 0, (hipStream_t)stream, b);
-    }
+    if (x_type == kU8) linear_launch<OT, true>(a, (hipStream_t)stream);
+    else linear_launch<OT, false>(a, (hipStream_t)stream);
     return 0;
   });
   return launched("tg_linear_i8");
@@ -152,7 +192,9 @@ int tg_quantize_i8(int device, void* stream, const void* x, int x_type, int64_t 
 
 int64_t tg_beam_select_workspace(int64_t groups, int64_t beams_in, int64_t vocab, int64_t beams_out) {
   if (groups < 0 || beams_in < 0 || vocab < 0 || beams_out < 0) return fail(TG_EINVAL, "tg_beam_select_workspace: negative size");
-  return 0;
+  if (groups == 0 || beams_in == 0 || vocab == 0) return 0;
+  const SelectPlan p = select_plan(groups, beams_in, vocab);
+  return p.small ? 0 : groups * beams_in * p.chunks * select_part_bytes((int)beams_out);
 }
 
 int tg_beam_select(int device, void* stream, const void* logits, int type, int64_t groups, int64_t beams_in, int64_t vocab, int64_t lg,
@@ -163,7 +205,7 @@ int tg_beam_select(int device, void* stream, const void* logits, int type, int64
   if (groups < 0 || groups > kMaxGrid) return fail(TG_EINVAL, "tg_beam_select: %lld groups", (long long)groups);
   if (beams_in < 1 || beams_in > TG_OPS_MAX_BEAMS || beams_out < 1 || beams_out > TG_OPS_MAX_BEAMS)
     return fail(TG_EINVAL, "tg_beam_select: %lld beams in, %lld out: 1 .. %d are supported", (long long)beams_in, (long long)beams_out, TG_OPS_MAX_BEAMS);
-  if (vocab < 1 || vocab > (1 << 24)) return fail(TG_EINVAL, "tg_beam_select: %lld entries: 1 .. 2^24 are supported", (long long)vocab);
+  if (vocab < 1 || vocab > TG_OPS_MAX_VOCAB) return fail(TG_EINVAL, "tg_beam_select: %lld entries: 1 .. %d are supported", (long long)vocab, TG_OPS_MAX_VOCAB);
   if (finished && (pad < 0 || pad >= vocab)) return fail(TG_EINVAL, "tg_beam_select: pad %d outside the %lld entries", pad, (long long)vocab);
   if (groups == 0) return TG_OK;
   if (lg < 0 || lk < 0 || lg > kMost || lk > kMost / 64 || (mask && (mg < 0 || mk < 0 || mg > kMost || mk > kMost / 64)))
@@ -171,6 +213,8 @@ int tg_beam_select(int device, void* stream, const void* logits, int type, int64
   if (!logits || !scores || !out_scores || !parents || !tokens) return fail(TG_EINVAL, "tg_beam_select: null pointer");
   if ((uintptr_t)logits % type_size(type) || (uintptr_t)scores % 4 || (uintptr_t)out_scores % 4 || (uintptr_t)parents % 4 || (uintptr_t)tokens % 4)
     return fail(TG_EINVAL, "tg_beam_select: an array is not aligned to its elements");
+  const SelectPlan p = select_plan(groups, beams_in, vocab);
+  if (!p.small && groups * beams_in * p.chunks > kMaxGrid) return fail(TG_EINVAL, "tg_beam_select: %lld groups x %lld beams x %lld entries: too much in one call", (long long)groups, (long long)beams_in, (long long)vocab);
   const int64_t need = tg_beam_select_workspace(groups, beams_in, vocab, beams_out);
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
     return fail(TG_EINVAL, "tg_beam_select: a 16-byte aligned workspace of %lld bytes is needed, got %lld", (long long)need, (long long)workspace_bytes);
@@ -188,7 +232,22 @@ int tg_beam_select(int device, void* stream, const void* logits, int type, int64
   const SelectArgs a{logits, scores, mask, finished, out_scores, parents, tokens, lg, lk, mg, mk, groups, (int)beams_in, (int)vocab, (int)beams_out, pad, normalize != 0};
   by_float(type, [&](auto e) {
     using T = decltype(e);
-    hipLaunchKernelGGL((select_scan_kernel<T>), dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, a);
+    const hipStream_t st = (hipStream_t)stream;
+    if (p.small) {
+      const dim3 grid((unsigned)((groups + 3) / 4));
+      if (p.per_lane <= 2) hipLaunchKernelGGL((select_small_kernel<T, 2>), grid, dim3(256), 0, st, a, p.shift);
+      else if (p.per_lane <= 5) hipLaunchKernelGGL((select_small_kernel<T, 5>), grid, dim3(256), 0, st, a, p.shift);
+      else if (p.per_lane <= 8) hipLaunchKernelGGL((select_small_kernel<T, 8>), grid, dim3(256), 0, st, a, p.shift);
+      else hipLaunchKernelGGL((select_small_kernel<T, 16>), grid, dim3(256), 0, st, a, p.shift);
+    } else {
+      const dim3 grid((unsigned)(groups * beams_in * p.chunks));
+      const size_t lds = (size_t)select_list((int)beams_out, p.e) * 8;  // (at most 64 KiB)
+      uint8_t* ws = (uint8_t*)workspace;
+      if (p.e == 8) hipLaunchKernelGGL((select_chunk_kernel<T, 8>), grid, dim3(256), lds, st, a, p.chunks, ws);
+      else if (p.e == 16) hipLaunchKernelGGL((select_chunk_kernel<T, 16>), grid, dim3(256), lds, st, a, p.chunks, ws);
+      else hipLaunchKernelGGL((select_chunk_kernel<T, 32>), grid, dim3(256), lds, st, a, p.chunks, ws);
+      hipLaunchKernelGGL(select_merge_kernel, dim3((unsigned)groups), dim3(64), 0, st, a, p.chunks, (const uint8_t*)ws);
+    }
     return 0;
   });
   return launched("tg_beam_select");
@@ -254,6 +313,29 @@ int tg_beam_reorder(int device, void* stream, int n, const void* const* src, voi
   ON_DEVICE("tg_beam_reorder", device);
   hipLaunchKernelGGL(reorder_kernel, dim3((p.items + 3) / 4), dim3(256), 0, (hipStream_t)stream, p);
   return launched("tg_beam_reorder");
+}
+
+int tg_beam_advance(int device, void* stream, int64_t groups, int64_t beams, const int32_t* parents, const int32_t* tokens,
+                    const float* gain_in, float* gain_out, int32_t* actions) {
+  if (groups < 0 || groups > kMaxGrid || beams < 1 || beams > TG_OPS_MAX_BEAMS)
+    return fail(TG_EINVAL, "tg_beam_advance: %lld groups of %lld beams", (long long)groups, (long long)beams);
+  const int64_t n = groups * beams;
+  if (n == 0) return TG_OK;
+  if (!parents || !tokens || !gain_in || !gain_out || !actions) return fail(TG_EINVAL, "tg_beam_advance: null pointer");
+  if (overlap(gain_out, 4 * n, gain_in, 4 * n)) return fail(TG_EINVAL, "tg_beam_advance: gain_out overlaps gain_in");
+  ON_DEVICE("tg_beam_advance", device);
+  hipLaunchKernelGGL(advance_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, parents, tokens, gain_in, gain_out,
+                     actions, n, (int)beams);
+  return launched("tg_beam_advance");
+}
+
+int tg_beam_collect(int device, void* stream, int64_t n, const tg_step_out* out, float* gain) {
+  if (n < 0 || n > kMaxGrid) return fail(TG_EINVAL, "tg_beam_collect: %lld environments", (long long)n);
+  if (n == 0) return TG_OK;
+  if (!out || !gain) return fail(TG_EINVAL, "tg_beam_collect: null pointer");
+  ON_DEVICE("tg_beam_collect", device);
+  hipLaunchKernelGGL(collect_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, out, gain, n);
+  return launched("tg_beam_collect");
 }
 
 }  // extern "C"
