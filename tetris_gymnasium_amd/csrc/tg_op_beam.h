@@ -19,25 +19,23 @@ struct SelectArgs {
   int k, v, beams, pad, norm;
 };
 
-// e^d for d <= 0 to 3e-13 of its value (NaN stays, far below zero gives 0): 2^n e^r with |r| <= ln(2)/2 and the exponential series to
-// r^10 (the next term is below 0.3466^11 / 11! = 2.2e-13).  n comes out of the low bits of d log2(e) + 1.5 * 2^52.
+// e^d for d <= 0 (or NaN: e^-700; the callers look for NaN themselves) to 1.1e-12 of its value, in 16 instructions: d log2(e) = n + f,
+// |f| <= 1/2; 2^f is the Chebyshev interpolation of degree 8 on [-1/2, 1/2], and n is added to its exponent.  Below -700 it stays at
+// 1e-304, which is nothing beside the largest term's 1.
 __device__ __forceinline__ double exp_neg(double d) {
-  d = d < -800.0 ? -800.0 : d;
-  const double big = 6755399441055744.0, z = fma(d, 1.4426950408889634, big), n = z - big;
-  double r = fma(-n, 0x1.62e42fefa0000p-1, d);  // ln 2 in two parts; n times the first (41 bits) is exact
-  r = fma(-n, 0x1.cf79abc9e3b3ap-41, r);
-  double p = 1.0 / 3628800;
-  p = fma(p, r, 1.0 / 362880);
-  p = fma(p, r, 1.0 / 40320);
-  p = fma(p, r, 1.0 / 5040);
-  p = fma(p, r, 1.0 / 720);
-  p = fma(p, r, 1.0 / 120);
-  p = fma(p, r, 1.0 / 24);
-  p = fma(p, r, 1.0 / 6);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  return ldexp(p, (int)(uint32_t)(uint64_t)__double_as_longlong(z));
+  const double big = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the nearest integer
+  const double t = fmax(d, -700.0) * 1.4426950408889634, z = t + big, f = t - (z - big);
+  double p = 0x1.63d1279ae38e4p-20;
+  p = fma(p, f, 0x1.00dc4a6dc0000p-16);
+  p = fma(p, f, 0x1.4308ac93a7c72p-13);
+  p = fma(p, f, 0x1.5d8745a6f2c72p-10);
+  p = fma(p, f, 0x1.3b2ab7181339fp-7);
+  p = fma(p, f, 0x1.c6b08dd6fd627p-5);
+  p = fma(p, f, 0x1.ebfbdff823d48p-3);
+  p = fma(p, f, 0x1.62e42fef84cedp-1);
+  p = fma(p, f, 1.0);
+  const uint64_t u = (uint64_t)__double_as_longlong(p);
+  return __longlong_as_double((long long)(u + ((uint64_t)(uint32_t)(uint64_t)__double_as_longlong(z) << 52)));
 }
 
 // A candidate as two words, larger = better, {0, .} = none: the score, then (beam, logit, entry) — within a beam the score never falls
@@ -64,43 +62,50 @@ __device__ __forceinline__ uint64_t lane_u64(uint64_t v, int l) {  // the value 
 }
 __device__ __forceinline__ uint64_t max_u64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
+__device__ __forceinline__ float lane_f32(float v, int l) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), l)); }
+
 // A bound that at least `beams` (or all) of the wave's lane maxima reach: with up to 16 beams the beams-th largest of the 16 maxima of
-// four lanes, else of the 64 lane maxima, by counting for each how many are larger.  Fewer than that: 1 (any candidate).
-__device__ __forceinline__ uint64_t wave_bound(uint64_t m, int beams) {
+// four lanes, else of the 64 lane maxima, by counting for each how many are larger.  m = -inf: the lane has nothing; none then passes
+// a bound above -inf.  For T = float and uint64_t.
+template <class T> __device__ __forceinline__ T wave_bound(T m, int beams, T (*lane)(T, int), T top) {
+  auto hi = [](T a, T b) { return a > b ? a : b; };
   const bool quads = beams <= 16;
-  if (quads) m = group_reduce<4>(m, max_u64);
+  if (quads) m = group_reduce<4>(m, hi);
   int larger = 0;
   if (quads) {
 #pragma unroll
-    for (int l = 0; l < 64; l += 4) larger += lane_u64(m, l) > m;
+    for (int l = 0; l < 64; l += 4) larger += lane(m, l) > m;
   } else {
-    for (int l = 0; l < 64; ++l) larger += lane_u64(m, l) > m;
+    for (int l = 0; l < 64; ++l) larger += lane(m, l) > m;
   }
   // of the values with fewer than `beams` larger ones the smallest: equal values count once, so this is never above the beams-th
-  const uint64_t low = group_reduce<64>(larger < beams ? m : ~(uint64_t)0, [](uint64_t a, uint64_t b) { return a < b ? a : b; });
-  return low ? low : 1;
+  return group_reduce<64>(larger < beams ? m : top, [](T a, T b) { return a < b ? a : b; });
 }
 
 // Of N candidates per lane the best `beams` of the wave, handed to put(rank, key) in descending order; returns how many there are.
-// What reaches the bound is packed into one candidate per lane through LDS (64 keys per wave) and ranked by counting; where more than
-// 64 reach it (many equal ones, many beams), the best is taken out `beams` times instead.
+// The bound is taken over the scores rounded to float32 (rounding keeps their order, so nothing that belongs to the best is lost);
+// what reaches it is packed into one candidate per lane through LDS (64 keys per wave) and ranked by counting; where more than 64
+// reach it (many equal ones, many beams), the best is taken out `beams` times instead.
 template <int N, class F> __device__ __forceinline__ int wave_top(Key (&k)[N], int beams, Key* lds, F put) {
   const int lane = threadIdx.x & 63;
-  uint64_t m = 0;
+  float c[N], m = -__builtin_inff();
 #pragma unroll
-  for (int i = 0; i < N; ++i) m = max_u64(m, k[i].s);
-  const uint64_t bound = wave_bound(m, beams);
+  for (int i = 0; i < N; ++i) {
+    c[i] = k[i].s ? fmaxf((float)unorder_f64(k[i].s), -3.402823466e38f) : -__builtin_inff();  // (a score below the float range is still one)
+    m = fmaxf(m, c[i]);
+  }
+  const float bound = fmaxf(wave_bound<float>(m, beams, lane_f32, __builtin_inff()), -3.402823466e38f);
   int n = 0, at[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const uint64_t b = __ballot(k[i].s >= bound);
+    const uint64_t b = __ballot(c[i] >= bound);
     at[i] = n + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
     n += (int)__popcll(b);
   }
   if (n <= 64) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (k[i].s >= bound) lds[at[i]] = k[i];
+      if (c[i] >= bound) lds[at[i]] = k[i];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     Key c = {0, 0};
@@ -170,8 +175,13 @@ template <class T, int N> __global__ __launch_bounds__(256) void select_small_ke
     if (L > 32) m = fm(m, xor_lane<32>(m));
     double s = 0;
     const double md = m;
+    bool nan = m == __builtin_inff();
 #pragma unroll
-    for (int i = 0; i < N; ++i) s += exp_neg((double)e[i] - md);  // (m = -inf, +inf or a NaN among them: NaN, no candidate)
+    for (int i = 0; i < N; ++i) {
+      nan |= e[i] != e[i];
+      s += exp_neg((double)e[i] - md);  // (m = -inf: the beam has no candidate, whatever this is)
+    }
+    if (nan) s = __builtin_nan("");  // (not a distribution: no candidate)
     if (L > 1) s += xor_lane<1>(s);
     if (L > 2) s += xor_lane<2>(s);
     if (L > 4) s += xor_lane<4>(s);
@@ -256,6 +266,7 @@ template <class T, int E> __global__ __launch_bounds__(256) void select_chunk_ke
 #pragma unroll
     for (int i = 0; i < E; ++i) s += exp_neg((double)e[i] - md);
     if (nan || m == __builtin_inff()) s = __builtin_nan("");
+    if (m == -__builtin_inff()) s = nan ? s : 0.0;
     s = group_reduce<64>(s, [](double p, double q) { return p + q; });
     if (lane == 0) wsum[wave] = s;
   }
@@ -267,14 +278,14 @@ template <class T, int E> __global__ __launch_bounds__(256) void select_chunk_ke
     if (e[i] == lm && lm > -__builtin_inff()) { best = i; bx = lm; }
   auto entry = [&](int i) { return v0 + (i / V) * 256 * V + i % V; };
   auto key = [&](float f, int v) { return f > -__builtin_inff() ? ((uint64_t)order_f32(f) << 32) | (uint32_t)~v : 0ull; };
-  const uint64_t bound = wave_bound(key(bx, entry(best)), a.beams);
-  const uint32_t bhi = (uint32_t)(bound >> 32);
+  const uint64_t bound = wave_bound<uint64_t>(key(bx, entry(best)), a.beams, lane_u64, ~(uint64_t)0);
+  const float bf = bound ? unorder_f32((uint32_t)(bound >> 32)) : -3.402823466e38f;
 #pragma unroll
   for (int i = 0; i < E; ++i) {
-    const bool maybe = e[i] > -__builtin_inff() && order_f32(e[i]) >= bhi;
+    const bool maybe = e[i] >= bf;
     if (__ballot(maybe)) {
       const uint64_t k = maybe ? key(e[i], entry(i)) : 0;
-      if (k >= bound) list[atomicAdd(&count, 1)] = k;
+      if (k && k >= bound) list[atomicAdd(&count, 1)] = k;
     }
   }
   __syncthreads();
@@ -288,77 +299,75 @@ template <class T, int E> __global__ __launch_bounds__(256) void select_chunk_ke
   if (t == 0) *head = {a.norm ? wsum[0] + wsum[1] + wsum[2] + wsum[3] : 0.0, m, keep};
 }
 
-// ... second step: a wave per group puts the chunks' sums and lists together.  Candidates come in rounds of 64 * 4, the first entries of
-// all lists before the second ones, so that later rounds soon hold nothing better than the `beams` already found.
-__global__ __launch_bounds__(64) void select_merge_kernel(const SelectArgs a, int chunks, const uint8_t* ws) {
-  constexpr int N = 4;
-  __shared__ Key lds[64], top[64];
+// ... second step: a workgroup per group puts the chunks' sums and lists together.  All heads are read at once, a lane per chunk; the
+// candidates come in rounds of 256, the first entries of all lists before the second ones, so that later rounds soon hold nothing
+// better than the `beams` already found.  A round goes through each of the four waves' own best to the first wave.
+__global__ __launch_bounds__(256) void select_merge_kernel(const SelectArgs a, int chunks, const uint8_t* ws) {
+  __shared__ Key lds[4][64], mine[4][64], top[64];
   __shared__ double lse[64];
-  const int lane = threadIdx.x;
+  __shared__ int have[4];
+  __shared__ Key bottom;  // the worst of the `beams` found so far, or none
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int64_t g = blockIdx.x, pb = select_part_bytes(a.beams);
   const uint8_t* base = ws + g * a.k * chunks * pb;
-  if (lane < a.k) {
-    double L = 0;
-    if (a.norm) {
-      float m = -__builtin_inff();
-      for (int c = 0; c < chunks; ++c) m = fmaxf(m, ((const SelectPart*)(base + ((int64_t)lane * chunks + c) * pb))->m);
-      double s = 0;
-      for (int c = 0; c < chunks; ++c) {
-        const SelectPart* h = (const SelectPart*)(base + ((int64_t)lane * chunks + c) * pb);
-        const double hs = h->s;
-        if (hs != 0.0) s += hs * exp_neg((double)h->m - (double)m);
-      }
-      L = (double)m + log(s);
-    }
-    lse[lane] = L;
-  }
-  int found = 0;
-  __syncthreads();
   const int lists = a.k * chunks;
   const int64_t total = (int64_t)lists * a.beams;
-  Key bottom = {0, 0};  // the worst of the `beams` found so far, or none
-  for (int64_t i0 = -64; i0 < total;) {
-    Key k[N];
-    bool any = false;
-    if (i0 < 0) {  // first the finished beams, a candidate each
-#pragma unroll
-      for (int i = 0; i < N; ++i) k[i] = {0, 0};
-      if (lane < a.k && a.finished && a.finished[g * a.k + lane]) {
-        k[0] = make_key((double)a.scores[g * a.k + lane], lane, 0, a.pad);
-        any = k[0].s != 0;
+  auto part = [&](int l) { return (const SelectPart*)(base + (int64_t)l * pb); };
+  if (a.norm) {  // a wave per beam, a lane per chunk
+    for (int j = wave; j < a.k; j += 4) {
+      float m = -__builtin_inff();
+      for (int c = lane; c < chunks; c += 64) m = fmaxf(m, part(j * chunks + c)->m);
+      m = group_reduce<64>(m, [](float p, float q) { return fmaxf(p, q); });
+      double s = 0;
+      for (int c = lane; c < chunks; c += 64) {
+        const SelectPart h = *part(j * chunks + c);
+        if (h.s != 0.0) s += h.s * exp_neg((double)h.m - (double)m);
       }
-      i0 = 0;
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int64_t c = i0 + i * 64 + lane;
-        k[i] = {0, 0};
-        if (c < total) {
-          const int rank = (int)(c / lists), l = (int)(c - (int64_t)rank * lists), row = l / chunks;
-          const uint8_t* part = base + (int64_t)l * pb;
-          if (rank < ((const SelectPart*)part)->n) {
-            const uint64_t u = ((const uint64_t*)(part + 16))[rank];
-            const float x = unorder_f32((uint32_t)(u >> 32));
-            k[i] = make_key((double)a.scores[g * a.k + row] + ((double)x - lse[row]), row, (uint32_t)(u >> 32), (int)~(uint32_t)u);
-            if (!better(k[i], bottom)) k[i].s = 0;
-            any |= k[i].s != 0;
-          }
-        }
-      }
-      i0 += 64 * N;
+      s = group_reduce<64>(s, [](double p, double q) { return p + q; });
+      if (lane == 0) lse[j] = (double)m + log(s);
     }
-    if (!__ballot(any)) continue;
-    Key all[N + 1];
-#pragma unroll
-    for (int i = 0; i < N; ++i) all[i] = k[i];
-    all[N] = lane < found ? top[lane] : Key{0, 0};
-    __builtin_amdgcn_wave_barrier();
-    found = wave_top(all, a.beams, lds, [&](int rank, const Key& c) { top[rank] = c; });
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (found == a.beams) bottom = top[a.beams - 1];
+  } else if (t < a.k) {
+    lse[t] = 0;
   }
-  if (lane < a.beams) put_result(a, g * a.beams + lane, lane < found ? top[lane] : Key{0, 0});
+  if (t == 0) bottom = {0, 0};
+  int found = 0;
+  for (int64_t i0 = -1; i0 < total; i0 += i0 < 0 ? 1 : 256) {
+    Key k[1] = {{0, 0}};
+    uint64_t u = 0;
+    int row = 0;
+    if (i0 >= 0 && i0 + t < total) {
+      const int64_t c = i0 + t;
+      const int rank = (int)(c / lists), l = (int)(c - (int64_t)rank * lists);
+      row = l / chunks;
+      if (rank < part(l)->n) u = ((const uint64_t*)(part(l) + 1))[rank];
+    }
+    __syncthreads();  // (lse; the round before)
+    if (u) {
+      const float x = unorder_f32((uint32_t)(u >> 32));
+      k[0] = make_key((double)a.scores[g * a.k + row] + ((double)x - lse[row]), row, (uint32_t)(u >> 32), (int)~(uint32_t)u);
+    } else if (i0 < 0 && t < a.k && a.finished && a.finished[g * a.k + t]) {  // first the finished beams, a candidate each
+      k[0] = make_key((double)a.scores[g * a.k + t], t, 0, a.pad);
+    }
+    if (!better(k[0], bottom)) k[0].s = 0;
+    int n = 0;
+    if (__ballot(k[0].s != 0)) {
+      n = wave_top(k, a.beams, lds[wave], [&](int rank, const Key& c) { mine[wave][rank] = c; });
+    }
+    if (lane == 0) have[wave] = n;
+    __syncthreads();
+    if (wave == 0 && have[0] + have[1] + have[2] + have[3] > 0) {
+      Key all[5];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) all[i] = lane < have[i] ? mine[i][lane] : Key{0, 0};
+      all[4] = lane < found ? top[lane] : Key{0, 0};
+      __builtin_amdgcn_wave_barrier();
+      found = wave_top(all, a.beams, lds[0], [&](int rank, const Key& c) { top[rank] = c; });
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (found == a.beams && lane == 0) bottom = top[a.beams - 1];
+    }
+  }
+  if (t < a.beams) put_result(a, g * a.beams + t, t < found ? top[t] : Key{0, 0});  // (wave 0: beams <= 64)
 }
 
 // which of them, by sizes alone (the workspace goes by it)
@@ -383,7 +392,7 @@ inline SelectPlan select_plan(int64_t groups, int64_t k, int64_t v) {
 // An item is gp groups x kin beams x cb columns (units of 1 << shift bytes) of one array, at most 64 * kReg units: a wave takes the
 // whole item into registers before it stores any of it, and columns of a row do not depend on each other, so the rows of a group
 // may be permuted in place.
-constexpr int kReorderReg = 4, kReorderMax = 24;
+constexpr int kReorderReg = 8, kReorderMax = 24;
 struct ReorderArray {
   const uint8_t* src;
   uint8_t* dst;
@@ -392,7 +401,7 @@ struct ReorderArray {
   uint32_t first;                  // first item
   uint32_t blocks;                 // column blocks
   int cb, gp, shift;
-  uint32_t mul_cb, mul_out;        // t / cb = t * mul_cb >> 20, likewise / beams out (t < 256)
+  uint32_t mul_cb, mul_out;        // t / cb = t * mul_cb >> 21, likewise / beams out (t < 512)
 };
 struct ReorderArgs {
   ReorderArray a[kReorderMax];
@@ -409,8 +418,8 @@ template <class U> __device__ __forceinline__ void reorder_item(const ReorderArr
 #pragma unroll
   for (int i = 0; i < kReorderReg; ++i) {
     const uint32_t t = (uint32_t)(i * 64 + lane);
-    const uint32_t rg = (t * a.mul_cb) >> 20, c = t - rg * a.cb;        // row of the item, column
-    const uint32_t dg = (rg * a.mul_out) >> 20, r = rg - dg * p.kout;   // group of the item, beam
+    const uint32_t rg = (t * a.mul_cb) >> 21, c = t - rg * a.cb;        // row of the item, column
+    const uint32_t dg = (rg * a.mul_out) >> 21, r = rg - dg * p.kout;   // group of the item, beam
     const int64_t g = g0 + dg, col = c0 + c;
     to[i] = nullptr;
     if ((int)dg < a.gp && g < p.groups && col < a.units) {

@@ -19,7 +19,6 @@ struct LinearArgs {
   void* out;
   int64_t rows, k, n, x_stride, w_stride, out_stride;
   int relu;
-  int vec;  // 16-byte stores of the output are aligned
 };
 
 // 16 bytes of a row starting at byte k, zero behind the row's end (weights: what they hold there decides the sum)
@@ -44,13 +43,13 @@ template <class OT> __device__ __forceinline__ OT linear_out(int acc, float xs, 
 template <class OT, int N> __device__ __forceinline__ void linear_put(const LinearArgs& a, int64_t m, int64_t n, const OT (&y)[N]) {
   OT* o = (OT*)a.out + m * a.out_stride + n;
   constexpr int V = 16 / (int)sizeof(OT) < N ? 16 / (int)sizeof(OT) : N;
-  if (a.vec && n + N <= a.n) {
+  if (n + N <= a.n) {  // (vector stores at any address: rows of an odd width start anywhere)
 #pragma unroll
     for (int i = 0; i < N; i += V) {
-      struct alignas(V * sizeof(OT)) { OT e[V]; } v;
+      struct __attribute__((packed, aligned(1))) { OT e[V]; } v;
 #pragma unroll
       for (int j = 0; j < V; ++j) v.e[j] = y[i + j];
-      *(decltype(v)*)(o + i) = v;
+      __builtin_memcpy((void*)(o + i), &v, sizeof(v));
     }
   } else {
 #pragma unroll
@@ -72,6 +71,8 @@ template <class OT, int N> __device__ __forceinline__ void linear_store(const Li
 // Bound by memory: a byte of input is used N times, N <= a few hundred.  A wave keeps the weights of 64 columns in registers (16 KS
 // of them) and walks over tiles of 16 rows, the next tile's fragments in flight behind the present one's products.
 template <class OT, bool U8, int KS> __global__ __launch_bounds__(256) void linear_rows_kernel(const LinearArgs a, int strips) {
+  // C columns make 16 bytes of output, G tiles a lane's C columns: the four lanes of a row then store 64 bytes side by side at a time
+  constexpr int C = 16 / (int)sizeof(OT), G = C / 4;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
   const int64_t n0 = ((int64_t)blockIdx.y * strips + wave % strips) * 64;  // `strips` of the four waves side by side, the others below
   const int below = 4 / strips;
@@ -96,8 +97,8 @@ template <class OT, bool U8, int KS> __global__ __launch_bounds__(256) void line
   v4i w[KS][4], init[4] = {}, f[KS];
   fetch(tile, f);
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {  // place (tile t, row 4 p + i) of the fragment holds column 16 p + 4 t + i: lane (q, .) ends with 16 q .. 16 q + 15
-    const int64_t n = n0 + 16 * (r >> 2) + 4 * t + (r & 3);
+  for (int t = 0; t < 4; ++t) {  // place (tile t, row 4 p + i) of the fragment holds column 4 C (t / G) + C p + 4 (t % G) + i: see C
+    const int64_t n = n0 + 4 * C * (t / G) + C * (r >> 2) + 4 * (t % G) + (r & 3);
     const uint8_t* wr = (const uint8_t*)a.w + (n < a.n ? n : a.n - 1) * a.w_stride;
 #pragma unroll
     for (int s = 0; s < KS; ++s) w[s][t] = load16_row(wr, 64 * s + 16 * q, a.k);
@@ -112,11 +113,11 @@ template <class OT, bool U8, int KS> __global__ __launch_bounds__(256) void line
         init[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[s][t], c64, init[t], 0, 0, 0);
       }
   }
-  const int64_t nq = n0 + 16 * q;
   float ws[16], b[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const int64_t c = nq + i < a.n ? nq + i : a.n - 1;
+    int64_t c = n0 + 4 * C * (i / C) + C * q + i % C;
+    c = c < a.n ? c : a.n - 1;
     ws[i] = a.ws[c];
     b[i] = a.bias ? a.bias[c] : 0.0f;
   }
@@ -137,10 +138,13 @@ template <class OT, bool U8, int KS> __global__ __launch_bounds__(256) void line
       for (int t = 0; t < 4; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[s][t], f[s], acc[t], 0, 0, 0);
     }
     if (m < a.rows) {
-      OT y[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) y[i] = linear_out<OT>(acc[i >> 2][i & 3], xs, ws[i], b[i], a.relu);
-      linear_put<OT, 16>(a, m, nq, y);
+      for (int j = 0; j < 16; j += C) {
+        OT y[C];
+#pragma unroll
+        for (int i = 0; i < C; ++i) y[i] = linear_out<OT>(acc[(i + j) >> 2][(i + j) & 3], xs, ws[i + j], b[i + j], a.relu);
+        linear_put<OT, C>(a, m, n0 + 4 * j + C * q, y);
+      }
     }
     if (next >= tiles) return;
     tile = next;

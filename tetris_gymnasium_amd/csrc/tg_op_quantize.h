@@ -32,15 +32,74 @@ template <class T> __device__ __forceinline__ QVec<T> q_load(const T* row, int64
   return r;
 }
 
-struct QScale { float s, inv, half; bool ok; };
-__device__ __forceinline__ int q_round(float x, const QScale& c) {
+struct QScale { float s, inv, half; };
+// exactly: the neighbour decided by the remainder, halves to even
+__device__ __forceinline__ uint32_t q_exact(float x, const QScale& c) {
   float n = rintf(x * c.inv);
   n = fminf(fmaxf(n, -127.0f), 127.0f);  // (before the check: an overshoot of the estimate at +-127 is undone here)
   const float r = fmaf(-n, c.s, x);      // exact
   const bool odd = ((int)n & 1) != 0;
   if (r > c.half || (r == c.half && odd)) n += 1.0f;
   else if (r < -c.half || (r == -c.half && odd)) n -= 1.0f;
-  return c.ok ? (int)n : 0;
+  return (uint32_t)(int)n & 255u;
+}
+// Four at a time: with 1.5 * 2^23 added the estimate lies in the low byte of the float's bits, and it is right wherever the remainder
+// is below half a step — almost always; the rest of the wave's vector goes the exact way.
+__device__ __forceinline__ uint32_t q_round4(const float (&x)[4], const QScale& c) {
+  const float magic = 12582912.0f;
+  float y[4];
+  bool close = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    y[i] = fmaf(x[i], c.inv, magic);
+    close |= !(fabsf(fmaf(-(y[i] - magic), c.s, x[i])) < c.half);
+  }
+  if (__builtin_expect(__ballot(close) != 0, 0)) return q_exact(x[0], c) | (q_exact(x[1], c) << 8) | (q_exact(x[2], c) << 16) | (q_exact(x[3], c) << 24);
+  const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(y[1]), __float_as_uint(y[0]), 0x0C0C0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(y[3]), __float_as_uint(y[2]), 0x04000C0Cu);
+  return lo | hi;
+}
+
+// the largest |x| of a vector, as bits of the type (NaN and infinity compare above every finite value), joined with `top`
+template <class T> __device__ __forceinline__ uint32_t q_top(const QVec<T>& e, uint32_t top) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t b = __float_as_uint(e.v[j]) & 0x7FFFFFFFu;
+      top = top > b ? top : b;
+    }
+  } else {  // two 16-bit maxima side by side
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    uint32_t w[4];
+    __builtin_memcpy(w, &e, 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t b = w[j] & 0x7FFF7FFFu;
+      u16x2 p, q;
+      __builtin_memcpy(&p, &b, 4);
+      __builtin_memcpy(&q, &top, 4);
+      const u16x2 m = __builtin_elementwise_max(p, q);
+      __builtin_memcpy(&top, &m, 4);
+    }
+  }
+  return top;
+}
+// ... its value; NaN or infinity where the row holds one
+template <class T> __device__ __forceinline__ float q_top_value(uint32_t top) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(top);
+  else {
+    const uint16_t b = (uint16_t)((top >> 16) > (top & 0xFFFFu) ? top >> 16 : top);
+    T v;
+    __builtin_memcpy(&v, &b, 2);
+    return to_f32(v);
+  }
+}
+template <class T> __device__ __forceinline__ uint32_t q_top_join(uint32_t a, uint32_t b) {
+  if constexpr (sizeof(T) == 4) return a > b ? a : b;
+  else {
+    const uint32_t lo = (a & 0xFFFFu) > (b & 0xFFFFu) ? a & 0xFFFFu : b & 0xFFFFu, hi = (a >> 16) > (b >> 16) ? a >> 16 : b >> 16;
+    return lo | (hi << 16);
+  }
 }
 
 // LPR lanes per row (16, 64: rows share a wave / a row each; 256: a workgroup a row), NV loads held per lane
@@ -53,54 +112,45 @@ template <class T, int LPR, int NV> __global__ __launch_bounds__(256) void quant
   const int64_t rr = row < rows ? row : rows - 1;  // (lanes of a row beyond the last repeat it and store nothing)
   const T* xr = x + rr * xs;
   QVec<T> h[NV];
-  uint32_t top = 0;  // max |x| as bits: NaN and infinity compare above every finite value
+  uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int64_t k = ((int64_t)i * LPR + l) * V;
     h[i] = q_load(xr, k < K ? k : K, K);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const uint32_t b = __float_as_uint(to_f32(h[i].v[j])) & 0x7FFFFFFFu;
-      top = top > b ? top : b;
-    }
+    top = q_top<T>(h[i], top);
   }
-  for (int64_t k = ((int64_t)NV * LPR + l) * V; k < K; k += LPR * V) {
-    const QVec<T> e = q_load(xr, k, K);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const uint32_t b = __float_as_uint(to_f32(e.v[j])) & 0x7FFFFFFFu;
-      top = top > b ? top : b;
-    }
-  }
-  top = group_reduce<(LPR < 64 ? LPR : 64)>(top, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+  for (int64_t k = ((int64_t)NV * LPR + l) * V; k < K; k += LPR * V) top = q_top<T>(q_load(xr, k, K), top);
+  top = group_reduce<(LPR < 64 ? LPR : 64)>(top, q_top_join<T>);
   if constexpr (LPR > 64) {
     __shared__ uint32_t sh[LPR / 64];
     if ((t & 63) == 0) sh[t >> 6] = top;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < LPR / 64; ++i) top = top > sh[i] ? top : sh[i];
+    for (int i = 0; i < LPR / 64; ++i) top = q_top_join<T>(top, sh[i]);
   }
+  const float most = q_top_value<T>(top);
+  const bool ok = most < __builtin_inff();
   QScale c;
-  c.ok = top < 0x7F800000u;
-  c.s = fmaxf(__uint_as_float(top) / 127.0f, 0x1p-126f);
-  if (!c.ok) c.s = __uint_as_float(0x7FC00000u);
-  c.inv = 1.0f / c.s;
+  c.s = ok ? fmaxf(most / 127.0f, 0x1p-126f) : __uint_as_float(0x7FC00000u);
+  c.inv = ok ? 1.0f / c.s : 0.0f;
   c.half = 0.5f * c.s;
   if (row >= rows) return;
   if (l == 0) scale[row] = c.s;
   int8_t* qr = q + row * qs;
   auto put = [&](int64_t k, const QVec<T>& e) {
-    if (k + V <= K) {
-      uint32_t w[V / 4];
+    uint32_t w[V / 4];
 #pragma unroll
-      for (int j = 0; j < V / 4; ++j)
-        w[j] = (uint32_t)(q_round(to_f32(e.v[4 * j]), c) & 255) | ((uint32_t)(q_round(to_f32(e.v[4 * j + 1]), c) & 255) << 8) |
-               ((uint32_t)(q_round(to_f32(e.v[4 * j + 2]), c) & 255) << 16) | ((uint32_t)(q_round(to_f32(e.v[4 * j + 3]), c) & 255) << 24);
+    for (int j = 0; j < V / 4; ++j) {
+      const float x[4] = {to_f32(e.v[4 * j]), to_f32(e.v[4 * j + 1]), to_f32(e.v[4 * j + 2]), to_f32(e.v[4 * j + 3])};
+      w[j] = q_round4(x, c);
+      w[j] = ok ? w[j] : 0;
+    }
+    if (k + V <= K) {
       __builtin_memcpy(qr + k, w, V);
     } else {
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (k + j < K) qr[k + j] = (int8_t)q_round(to_f32(e.v[j]), c);
+        if (k + j < K) qr[k + j] = (int8_t)(w[j / 4] >> (8 * (j % 4)));
     }
   };
 #pragma unroll

@@ -71,8 +71,8 @@ template <class OT, bool U8, int KS> void linear_rows(const LinearArgs& a, hipSt
   const int64_t cols = (a.n + 63) / 64;
   const int strips = cols >= 4 ? 4 : cols == 2 ? 2 : 1, below = 4 / strips;
   const int64_t gy = (cols + strips - 1) / strips, tiles = (a.rows + 15) / 16;
-  // as many workgroups as stay resident (two per unit for the widest variant), each with a run of tiles
-  int64_t gx = (kUnits * 4 + gy - 1) / gy;
+  // as many workgroups as stay resident (by the variant's registers), each with a run of tiles
+  int64_t gx = (kUnits * (KS == 1 ? 3 : 2) + gy - 1) / gy;
   if (gx > (tiles + below - 1) / below) gx = (tiles + below - 1) / below;
   hipLaunchKernelGGL((linear_rows_kernel<OT, U8, KS>), dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, st, a, strips);
 }
@@ -144,8 +144,7 @@ int tg_linear_i8(int device, void* stream, const void* x, int x_type, int64_t ro
       overlap(out, no, x_scale, 4 * rows) || overlap(out, no, bias, 4 * n))
     return fail(TG_EINVAL, "tg_linear_i8: the output overlaps an input");
   ON_DEVICE("tg_linear_i8", device);
-  LinearArgs a{(const uint8_t*)x, w, w_scale, x_scale, bias, out, rows, k, n, x_stride, w_stride, out_stride, relu != 0,
-               (uintptr_t)out % 16 == 0 && (out_stride * os) % 16 == 0};
+  LinearArgs a{(const uint8_t*)x, w, w_scale, x_scale, bias, out, rows, k, n, x_stride, w_stride, out_stride, relu != 0};
   by_float(out_type, [&](auto o) {
     using OT = decltype(o);
     if (x_type == kU8) linear_launch<OT, true>(a, (hipStream_t)stream);
@@ -246,7 +245,7 @@ int tg_beam_select(int device, void* stream, const void* logits, int type, int64
       if (p.e == 8) hipLaunchKernelGGL((select_chunk_kernel<T, 8>), grid, dim3(256), lds, st, a, p.chunks, ws);
       else if (p.e == 16) hipLaunchKernelGGL((select_chunk_kernel<T, 16>), grid, dim3(256), lds, st, a, p.chunks, ws);
       else hipLaunchKernelGGL((select_chunk_kernel<T, 32>), grid, dim3(256), lds, st, a, p.chunks, ws);
-      hipLaunchKernelGGL(select_merge_kernel, dim3((unsigned)groups), dim3(64), 0, st, a, p.chunks, (const uint8_t*)ws);
+      hipLaunchKernelGGL(select_merge_kernel, dim3((unsigned)groups), dim3(256), 0, st, a, p.chunks, (const uint8_t*)ws);
     }
     return 0;
   });
@@ -295,8 +294,8 @@ int tg_beam_reorder(int device, void* stream, int n, const void* const* src, voi
     a.cb = (int)(a.units < most ? a.units : most);
     a.gp = (int)(64 * kReorderReg / (beams_out * a.cb));
     if (a.cb < a.units) a.gp = 1;
-    a.mul_cb = ((1u << 20) + a.cb - 1) / a.cb;
-    a.mul_out = ((1u << 20) + (uint32_t)beams_out - 1) / (uint32_t)beams_out;
+    a.mul_cb = ((1u << 21) + a.cb - 1) / a.cb;
+    a.mul_out = ((1u << 21) + (uint32_t)beams_out - 1) / (uint32_t)beams_out;
     const int64_t blocks = (a.units + a.cb - 1) / a.cb, items = blocks * ((groups + a.gp - 1) / a.gp);
     if (blocks > kMaxGrid || items + p.items > kMaxGrid) return fail(TG_EINVAL, "tg_beam_reorder: too much in one call (array %d)", i);
     a.blocks = (uint32_t)blocks;

@@ -31,7 +31,7 @@ class DeviceView:
     """A raw device pointer with a shape: dtype by name ("uint8", "int8", "bool", "int32", "float32", "float16", "bfloat16", ...),
     strides in elements (None = contiguous).  The caller keeps the memory alive."""
 
-    __slots__ = ("ptr", "shape", "dtype", "strides", "device")
+    __slots__ = ("ptr", "shape", "dtype", "strides", "device", "_meta")
 
     def __init__(self, ptr, shape, dtype, strides=None, device=0):
         if dtype not in _SIZES:
@@ -40,6 +40,7 @@ class DeviceView:
         self.strides = _contiguous(self.shape) if strides is None else tuple(int(s) for s in strides)
         if len(self.strides) != len(self.shape):
             raise ValueError("DeviceView: one stride per axis")
+        self._meta = (self.shape, self.strides, dtype, self.device)
 
 
 def _contiguous(shape):
@@ -50,19 +51,17 @@ def _contiguous(shape):
     return tuple(reversed(st))
 
 
-def _view(a, what):
-    """(pointer, shape, strides in elements, dtype name, device or None)"""
-    if hasattr(a, "data_ptr"):  # a torch tensor (not imported here)
-        dt = a.dtype
-        name = _names.get(dt)
-        if name is None:
-            name = _names[dt] = str(dt).rpartition(".")[2]
-        dev = a.device
-        if dev.type != "cuda":
-            raise ValueError(f"{what}: device memory is needed, got a tensor on {dev}")
-        return a.data_ptr(), tuple(a.shape), a.stride(), name, dev.index
+# An array comes in as (pointer, meta), meta = (shape, strides in elements, dtype, device): a call's metas decide everything that its
+# checks and the C entry's sizes depend on, so a call whose metas were seen before reuses their outcome (`_plans`) and only passes the
+# pointers on — the checks in Python cost more than a small kernel.  Pointers, values and objects are never kept.
+_plans: dict = {}
+
+
+def _get(a):
+    if hasattr(a, "data_ptr"):  # a torch tensor (torch is not imported here)
+        return a.data_ptr(), (a.shape, a.stride(), a.dtype, a.get_device())
     if isinstance(a, DeviceView):
-        return a.ptr, a.shape, a.strides, a.dtype, a.device
+        return a.ptr, a._meta
     if isinstance(a, DeviceArray):
         a._ready()
         name, item = a.dtype.name, a.dtype.itemsize
@@ -70,19 +69,47 @@ def _view(a, what):
             st = _contiguous(a.shape)
         else:
             if any(s % item for s in a.strides):
-                raise ValueError(f"{what}: strides are not whole elements")
+                raise ValueError("strides of a DeviceArray are not whole elements")
             st = tuple(s // item for s in a.strides)
-        return a.ptr, a.shape, st, name, int(a.engine.cfg.device)
+        return a.ptr, (a.shape, st, name, int(a.engine.cfg.device))
     cai = getattr(a, "__cuda_array_interface__", None)
     if cai is None:
-        raise ValueError(f"{what}: a device array is needed (torch tensor, DeviceArray, DeviceView or __cuda_array_interface__), got {type(a).__name__}")
+        raise ValueError(f"a device array is needed (torch tensor, DeviceArray, DeviceView or __cuda_array_interface__), got {type(a).__name__}")
     name = _STR.get(cai["typestr"])
     if name is None:
-        raise ValueError(f"{what}: unsupported element type {cai['typestr']}")
+        raise ValueError(f"unsupported element type {cai['typestr']}")
     shape, item = tuple(cai["shape"]), _SIZES[name]
     st = cai.get("strides")
     st = _contiguous(shape) if st is None else tuple(s // item for s in st)
-    return cai["data"][0], shape, st, name, None
+    return cai["data"][0], (shape, st, name, None)
+
+
+def _parse(meta, what):
+    """(shape, strides, dtype name, device or None) of a meta"""
+    shape, st, dt, dev = meta
+    if not isinstance(dt, str):
+        name = _names.get(dt)
+        if name is None:
+            name = _names[dt] = str(dt).rpartition(".")[2]
+        dt = name
+        if dev is not None and dev < 0:
+            raise ValueError(f"{what}: device memory is needed, got a tensor on the host")
+    return tuple(shape), tuple(st), dt, dev
+
+
+def _view(a, what):
+    p, meta = _get(a)
+    return (p, *_parse(meta, what))
+
+
+def _plan(key, make, *args):
+    plan = _plans.get(key)
+    if plan is None:
+        plan = make(*args)
+        if len(_plans) >= 4096:
+            _plans.clear()
+        _plans[key] = plan
+    return plan
 
 
 def _device(*devs):
@@ -93,7 +120,7 @@ def _device(*devs):
 
 
 def _lib():
-    lib = N.load()
+    lib = N._lib or N.load()
     if not N.HAVE_OPS:
         raise EngineError(f"{N.LIB_PATH} holds no operators (include/tetris_gym_ops.h): build the product library")
     return lib
@@ -153,38 +180,49 @@ def linear_i8(x, weight, weight_scale, out, *, x_scale=None, bias=None, relu=Fal
     x uint8 / int8 [..., K] (rows at any stride and alignment: the engine's boards and feature vectors as they lie), weight int8
     [N, K], weight_scale float32 [N], x_scale float32 [rows] or None (1), bias float32 [N] or None, out float32 / float16 /
     bfloat16 [..., N].  The sum is exact (K <= 65 536), the rest float32, rounded once; `relu` clips at zero.  Returns out."""
-    xp, xsh, xst, xt, d0 = _view(x, "linear_i8: x")
-    wp, wsh, wst, wt, d1 = _view(weight, "linear_i8: weight")
-    sp, ssh, sst, stt, d2 = _view(weight_scale, "linear_i8: weight_scale")
-    op, osh, ost, ot, d3 = _view(out, "linear_i8: out")
+    xp, xm = _get(x)
+    wp, wm = _get(weight)
+    sp, sm = _get(weight_scale)
+    op, om = _get(out)
+    xsp, xsm = (None, None) if x_scale is None else _get(x_scale)
+    bp, bm = (None, None) if bias is None else _get(bias)
+    dev, xtype, rows, k, xs, n, wst, otype, os_ = _plan(("linear", xm, wm, sm, om, xsm, bm), _linear_plan, xm, wm, sm, om, xsm, bm)
+    lib = _lib()
+    rc = lib.tg_linear_i8(dev, stream, xp, xtype, rows, k, xs, wp, n, wst, sp, xsp, bp, 1 if relu else 0, op, otype, os_)
+    if rc:
+        _check(lib, rc, "tg_linear_i8")
+    return out
+
+
+def _linear_plan(xm, wm, sm, om, xsm, bm):
+    xsh, xst, xt, d0 = _parse(xm, "linear_i8: x")
+    wsh, wst, wt, d1 = _parse(wm, "linear_i8: weight")
+    ssh, sst, stt, d2 = _parse(sm, "linear_i8: weight_scale")
+    osh, ost, ot, d3 = _parse(om, "linear_i8: out")
     xtype = _type(xt, "linear_i8: x", ("uint8", "int8"))
     _type(wt, "linear_i8: weight", ("int8",))
     _type(stt, "linear_i8: weight_scale", ("float32",))
     otype = _type(ot, "linear_i8: out", _FLOATS)
     rows, k, xs = _rows(xsh, xst, "linear_i8: x")
     orows, n, os_ = _rows(osh, ost, "linear_i8: out")
-    if len(wsh) != 2 or wsh != (n, k):
-        raise ValueError(f"linear_i8: weight must have shape {(n, k)}, got {tuple(wsh)}")
+    if wsh != (n, k):
+        raise ValueError(f"linear_i8: weight must have shape {(n, k)}, got {wsh}")
     _inner(wsh, wst, "linear_i8: weight")
     if orows != rows:
         raise ValueError(f"linear_i8: out has {orows} rows, x has {rows}")
     _dense(ssh, sst, (n,), "linear_i8: weight_scale")
     devs = [d0, d1, d2, d3]
-    p_xs = p_b = None
-    if x_scale is not None:
-        p_xs, sh, st, t, d = _view(x_scale, "linear_i8: x_scale")
+    if xsm is not None:
+        sh, st, t, d = _parse(xsm, "linear_i8: x_scale")
         _type(t, "linear_i8: x_scale", ("float32",))
         _dense(sh, st, (rows,) if len(sh) == 1 else xsh[:-1], "linear_i8: x_scale")
         devs.append(d)
-    if bias is not None:
-        p_b, sh, st, t, d = _view(bias, "linear_i8: bias")
+    if bm is not None:
+        sh, st, t, d = _parse(bm, "linear_i8: bias")
         _type(t, "linear_i8: bias", ("float32",))
         _dense(sh, st, (n,), "linear_i8: bias")
         devs.append(d)
-    lib = _lib()
-    _check(lib, lib.tg_linear_i8(_device(*devs), stream, xp, xtype, rows, k, xs, wp, n, wst[0], sp, p_xs, p_b, bool(relu), op, otype, os_),
-           "tg_linear_i8")
-    return out
+    return _device(*devs), xtype, rows, k, xs, n, wst[0], otype, os_
 
 
 def quantize_i8(x, q, scale, *, stream=0):
@@ -192,20 +230,30 @@ def quantize_i8(x, q, scale, *, stream=0):
 
     x float32 / float16 / bfloat16 [..., K], q int8 [..., K], scale float32 [rows].  q * scale is x to half a step.  A row with a
     NaN or an infinity gets scale NaN and q 0: what is computed from it is NaN, not a plausible number.  Returns (q, scale)."""
-    xp, xsh, xst, xt, d0 = _view(x, "quantize_i8: x")
-    qp, qsh, qst, qt, d1 = _view(q, "quantize_i8: q")
-    sp, ssh, sst, stt, d2 = _view(scale, "quantize_i8: scale")
+    xp, xm = _get(x)
+    qp, qm = _get(q)
+    sp, sm = _get(scale)
+    dev, xtype, rows, k, xs, qs = _plan(("quantize", xm, qm, sm), _quantize_plan, xm, qm, sm)
+    lib = _lib()
+    rc = lib.tg_quantize_i8(dev, stream, xp, xtype, rows, k, xs, qp, qs, sp)
+    if rc:
+        _check(lib, rc, "tg_quantize_i8")
+    return q, scale
+
+
+def _quantize_plan(xm, qm, sm):
+    xsh, xst, xt, d0 = _parse(xm, "quantize_i8: x")
+    qsh, qst, qt, d1 = _parse(qm, "quantize_i8: q")
+    ssh, sst, stt, d2 = _parse(sm, "quantize_i8: scale")
     xtype = _type(xt, "quantize_i8: x", _FLOATS)
     _type(qt, "quantize_i8: q", ("int8",))
     _type(stt, "quantize_i8: scale", ("float32",))
     rows, k, xs = _rows(xsh, xst, "quantize_i8: x")
-    if tuple(qsh) != tuple(xsh) and _rows(qsh, qst, "quantize_i8: q")[:2] != (rows, k):
-        raise ValueError(f"quantize_i8: q must have x's shape {tuple(xsh)}, got {tuple(qsh)}")
-    _, _, qs = _rows(qsh, qst, "quantize_i8: q")
+    qrows, qk, qs = _rows(qsh, qst, "quantize_i8: q")
+    if (qrows, qk) != (rows, k):
+        raise ValueError(f"quantize_i8: q must have x's shape {xsh}, got {qsh}")
     _dense(ssh, sst, (rows,) if len(ssh) == 1 else xsh[:-1], "quantize_i8: scale")
-    lib = _lib()
-    _check(lib, lib.tg_quantize_i8(_device(d0, d1, d2), stream, xp, xtype, rows, k, xs, qp, qs, sp), "tg_quantize_i8")
-    return q, scale
+    return _device(d0, d1, d2), xtype, rows, k, xs, qs
 
 
 def beam_select_workspace(groups, beams_in, vocab, beams_out):
@@ -228,18 +276,35 @@ def beam_select(logits, scores, out_scores, parents, tokens, *, mask=None, finis
     (beam, entry).  Missing ones: -inf, -1, -1.  logits float32 / float16 / bfloat16 [G, K, V].  `workspace`: uint8 memory of
     beam_select_workspace(G, K, V, B) bytes, not shared with a call that may run at the same time.
     Returns (out_scores, parents, tokens)."""
-    lp, lsh, lst, lt, d0 = _view(logits, "beam_select: logits")
-    sp, ssh, sst, stt, d1 = _view(scores, "beam_select: scores")
-    op, osh, ost, ot, d2 = _view(out_scores, "beam_select: out_scores")
-    pp, psh, pst, pt, d3 = _view(parents, "beam_select: parents")
-    tp, tsh, tst, tt, d4 = _view(tokens, "beam_select: tokens")
+    lp, lm = _get(logits)
+    sp, sm = _get(scores)
+    op, om = _get(out_scores)
+    pp, pm = _get(parents)
+    tp, tm = _get(tokens)
+    mp, mm = (None, None) if mask is None else _get(mask)
+    fp, fm = (None, None) if finished is None else _get(finished)
+    wp, wm = (None, None) if workspace is None else _get(workspace)
+    dev, ltype, g, k, v, lg, lk, mg, mk, b, nws = _plan(("select", lm, sm, om, pm, tm, mm, fm, wm), _select_plan, lm, sm, om, pm, tm, mm, fm, wm)
+    lib = _lib()
+    rc = lib.tg_beam_select(dev, stream, lp, ltype, g, k, v, lg, lk, sp, mp, mg, mk, fp, pad, 1 if normalize else 0, b, op, pp, tp, wp, nws)
+    if rc:
+        _check(lib, rc, "tg_beam_select")
+    return out_scores, parents, tokens
+
+
+def _select_plan(lm, sm, om, pm, tm, mm, fm, wm):
+    lsh, lst, lt, d0 = _parse(lm, "beam_select: logits")
+    ssh, sst, stt, d1 = _parse(sm, "beam_select: scores")
+    osh, ost, ot, d2 = _parse(om, "beam_select: out_scores")
+    psh, pst, pt, d3 = _parse(pm, "beam_select: parents")
+    tsh, tst, tt, d4 = _parse(tm, "beam_select: tokens")
     ltype = _type(lt, "beam_select: logits", _FLOATS)
     _type(stt, "beam_select: scores", ("float32",))
     _type(ot, "beam_select: out_scores", ("float32",))
     _type(pt, "beam_select: parents", ("int32",))
     _type(tt, "beam_select: tokens", ("int32",))
     if len(lsh) != 3 or len(osh) != 2:
-        raise ValueError(f"beam_select: logits must be [G, K, V] and out_scores [G, B], got {tuple(lsh)} and {tuple(osh)}")
+        raise ValueError(f"beam_select: logits must be [G, K, V] and out_scores [G, B], got {lsh} and {osh}")
     g, k, v = lsh
     b = osh[1]
     if not (1 <= k <= MAX_BEAMS and 1 <= b <= MAX_BEAMS and v >= 1):
@@ -249,38 +314,34 @@ def beam_select(logits, scores, out_scores, parents, tokens, *, mask=None, finis
     for sh, st, what in ((osh, ost, "out_scores"), (psh, pst, "parents"), (tsh, tst, "tokens")):
         _dense(sh, st, (g, b), "beam_select: " + what)
     devs = [d0, d1, d2, d3, d4]
-    mp = fp = wp = None
     mst = (0, 0)
-    if mask is not None:
-        mp, sh, mst, t, d = _view(mask, "beam_select: mask")
+    if mm is not None:
+        sh, mst, t, d = _parse(mm, "beam_select: mask")
         _type(t, "beam_select: mask", ("uint8", "bool"))
-        if tuple(sh) != (g, k, v):
-            raise ValueError(f"beam_select: mask must have shape {(g, k, v)}, got {tuple(sh)}")
+        if sh != (g, k, v):
+            raise ValueError(f"beam_select: mask must have shape {(g, k, v)}, got {sh}")
         _inner(sh, mst, "beam_select: mask")
         devs.append(d)
-    if finished is not None:
-        fp, sh, st, t, d = _view(finished, "beam_select: finished")
+    if fm is not None:
+        sh, st, t, d = _parse(fm, "beam_select: finished")
         _type(t, "beam_select: finished", ("uint8", "bool"))
         _dense(sh, st, (g, k), "beam_select: finished")
         devs.append(d)
     nws = 0
-    if workspace is not None:
-        wp, sh, st, t, d = _view(workspace, "beam_select: workspace")
+    if wm is not None:
+        sh, st, t, d = _parse(wm, "beam_select: workspace")
         _type(t, "beam_select: workspace", ("uint8",))
         if len(sh) != 1:
             raise ValueError("beam_select: workspace must have one axis")
         _dense(sh, st, sh, "beam_select: workspace")
         nws = sh[0]
         devs.append(d)
-    lib = _lib()
-    _check(lib, lib.tg_beam_select(_device(*devs), stream, lp, ltype, g, k, v, lst[0], lst[1], sp, mp, mst[0], mst[1], fp, pad, bool(normalize), b,
-                                   op, pp, tp, wp, nws), "tg_beam_select")
-    return out_scores, parents, tokens
+    return _device(*devs), ltype, g, k, v, lst[0], lst[1], mst[0], mst[1], b, nws
 
 
-def _state(a, rows, what):
-    """(pointer, bytes of a row, stride of a row in bytes, device) of [G * K, ...] or [G, K, ...]"""
-    p, sh, st, t, d = _view(a, what)
+def _state(meta, rows, what):
+    """(bytes of a row, stride of a row in bytes, device) of [G * K, ...] or [G, K, ...]"""
+    sh, st, t, d = _parse(meta, what)
     if t not in _SIZES:
         raise ValueError(f"{what}: unsupported element type {t}")
     lead, n = 0, 1
@@ -296,7 +357,7 @@ def _state(a, rows, what):
         cols *= k
     flat = _rows(tuple(sh[:lead]) + (1,), tuple(st[:lead]) + (1,), what)
     stride = flat[2] if flat[0] > 1 else cols
-    return p, cols * size, stride * size, d
+    return cols * size, stride * size, d
 
 
 def beam_reorder(states, parents, *, out=None, beams_in=None, stream=0):
@@ -306,39 +367,45 @@ def beam_reorder(states, parents, *, out=None, beams_in=None, stream=0):
     them.  K = beams_in, by default B.  out: the same number of arrays with B rows per group (not overlapping states), or None to
     reorder in place (B = K).
     A parent outside 0 .. K - 1 (the -1 of a missing beam) leaves its row as it was.  Returns out (or states)."""
-    single = not isinstance(states, (list, tuple))
-    src = [states] if single else list(states)
-    if out is None:
-        dst = src
-    else:
-        dst = list(out) if isinstance(out, (list, tuple)) else [out]
-        if len(dst) != len(src):
-            raise ValueError(f"beam_reorder: {len(src)} states, {len(dst)} outputs")
-    if len(src) > MAX_STATES:
-        raise ValueError(f"beam_reorder: {len(src)} arrays: up to {MAX_STATES} go into one call")
-    pp, psh, pst, pt, dev = _view(parents, "beam_reorder: parents")
+    src = states if isinstance(states, (list, tuple)) else (states,)
+    pp, pm = _get(parents)
+    sv = [_get(a) for a in src]
+    dv = sv if out is None else [_get(a) for a in (out if isinstance(out, (list, tuple)) else (out,))]
+    metas = tuple([m for _, m in sv])
+    outs = None if out is None else tuple([m for _, m in dv])
+    n, dev, g, k, b, ptrs, rows, ss, ds = _plan(("reorder", pm, metas, outs, beams_in), _reorder_plan, pm, metas, outs, beams_in)
+    if n and g:
+        lib = _lib()
+        rc = lib.tg_beam_reorder(dev, stream, n, ptrs(*[p for p, _ in sv]), ptrs(*[p for p, _ in dv]), rows, ss, ds, g, k, b, pp)
+        if rc:
+            _check(lib, rc, "tg_beam_reorder")
+    return states if out is None else out
+
+
+def _reorder_plan(pm, metas, outs, beams_in):
+    n = len(metas)
+    if outs is not None and len(outs) != n:
+        raise ValueError(f"beam_reorder: {n} states, {len(outs)} outputs")
+    if n > MAX_STATES:
+        raise ValueError(f"beam_reorder: {n} arrays: up to {MAX_STATES} go into one call")
+    psh, pst, pt, dev = _parse(pm, "beam_reorder: parents")
     _type(pt, "beam_reorder: parents", ("int32",))
     if len(psh) != 2:
-        raise ValueError(f"beam_reorder: parents must be [G, B], got {tuple(psh)}")
+        raise ValueError(f"beam_reorder: parents must be [G, B], got {psh}")
     _dense(psh, pst, psh, "beam_reorder: parents")
     g, b = psh
-    n = len(src)
-    if n == 0 or g == 0:
-        return states if out is None else out
     k = b if beams_in is None else int(beams_in)
     if not (1 <= k <= MAX_BEAMS and 1 <= b <= MAX_BEAMS):
         raise ValueError(f"beam_reorder: {k} beams in, {b} out: 1 .. {MAX_BEAMS} are supported")
-    if out is None and k != b:
+    if outs is None and k != b:
         raise ValueError(f"beam_reorder: in place takes as many beams out ({b}) as in ({k})")
-    arr = C.c_void_p * n
     num = C.c_int64 * n
-    sv = [_state(a, g * k, f"beam_reorder: states[{i}]") for i, a in enumerate(src)]
-    dv = sv if out is None else [_state(a, g * b, f"beam_reorder: out[{i}]") for i, a in enumerate(dst)]
+    if g == 0:
+        return n, 0, g, k, b, C.c_void_p * n, num(), num(), num()
+    sv = [_state(m, g * k, f"beam_reorder: states[{i}]") for i, m in enumerate(metas)]
+    dv = sv if outs is None else [_state(m, g * b, f"beam_reorder: out[{i}]") for i, m in enumerate(outs)]
     for i, (s, d) in enumerate(zip(sv, dv)):
-        if s[1] != d[1]:
-            raise ValueError(f"beam_reorder: rows of states[{i}] hold {s[1]} bytes, of out[{i}] {d[1]}")
-    lib = _lib()
-    _check(lib, lib.tg_beam_reorder(_device(dev, *(s[3] for s in sv), *(d[3] for d in dv)), stream, n, arr(*(s[0] for s in sv)),
-                                    arr(*(d[0] for d in dv)), num(*(s[1] for s in sv)), num(*(s[2] for s in sv)), num(*(d[2] for d in dv)),
-                                    g, k, b, pp), "tg_beam_reorder")
-    return states if out is None else out
+        if s[0] != d[0]:
+            raise ValueError(f"beam_reorder: rows of states[{i}] hold {s[0]} bytes, of out[{i}] {d[0]}")
+    return (n, _device(dev, *(s[2] for s in sv), *(d[2] for d in dv)), g, k, b, C.c_void_p * n, num(*(s[0] for s in sv)), num(*(s[1] for s in sv)),
+            num(*(d[1] for d in dv)))
