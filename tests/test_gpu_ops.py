@@ -31,7 +31,8 @@ def linear_case(box, rows, k, n, xdt, odt, x_scale, bias, relu, seed, xpitch=Non
     ops.linear_i8(box.put(x, pitch=xpitch, before=xbefore), box.put(w, pitch=wpitch, before=wbefore), box.put(ws), out,
                   x_scale=None if xs is None else box.put(xs), bias=None if b is None else box.put(b), relu=relu, stream=box.stream)
     got = box.get(out).astype(np.float64)
-    acc = x.astype(np.float64) @ w.astype(np.float64).T if k else np.zeros((rows, n))
+    exact = np.float32 if k * 255 * 128 < 2**24 else np.float64  # (integers: sums below 2^24 are exact in float32 too)
+    acc = (x.astype(exact) @ w.astype(exact).T).astype(np.float64) if k else np.zeros((rows, n))
     p = acc * ws.astype(np.float64) * (1.0 if xs is None else xs.astype(np.float64)[:, None])
     y = p + (0.0 if b is None else b)
     # the sum to float32, the product of the scales, their product with the bias in one fma: 2^-24 of the product each of the first two
@@ -59,6 +60,18 @@ def test_linear_sizes_and_types(box, rows, k, n, xdt, odt):
 @pytest.mark.parametrize("xdt", ["uint8", "int8"])
 def test_linear_larger(box, rows, k, n, odt, xdt):
     linear_case(box, rows, k, n, xdt, odt, True, True, False, seed=rows + k + n)
+
+
+@pytest.mark.parametrize("rows,k,n,xdt,odt", [(4100, 528, 4000, "int8", "bfloat16"), (4096, 512, 4097, "uint8", "float32"), (4099, 560, 4096, "uint8", "float16"),
+                                              (8200, 272, 1024, "uint8", "bfloat16"), (8193, 400, 1001, "int8", "float32"), (4200, 304, 1010, "uint8", "float16"),
+                                              (2050, 400, 1000, "int8", "float16"), (1030, 288, 200, "uint8", "float32"), (65, 1024, 8200, "int8", "bfloat16"),
+                                              (50, 300, 8200, "uint8", "float16"), (33, 1024, 8192, "int8", "float32"), (20, 2000, 8200, "int8", "bfloat16"),
+                                              (32, 333, 8195, "uint8", "float32"), (9, 515, 8200, "uint8", "bfloat16"), (200, 800, 500, "uint8", "bfloat16"),
+                                              (256, 130, 1024, "int8", "float32"), (5000, 901, 300, "uint8", "float16"), (20000, 37, 130, "uint8", "bfloat16"),
+                                              (20000, 128, 63, "int8", "float16"), (9000, 250, 777, "uint8", "float32"), (9000, 256, 40, "int8", "float32")])
+def test_linear_every_variant(box, rows, k, n, xdt, odt):
+    """sizes on both sides of the rules that choose a kernel: wide, medium and small tiles, few rows of many columns, short rows"""
+    linear_case(box, rows, k, n, xdt, odt, rows % 2 == 0, True, n % 2 == 0, seed=rows + n)
 
 
 @pytest.mark.parametrize("rows,k,n", [(40, 200, 70), (300, 256, 300), (9, 1024, 64), (260, 640, 130)])
@@ -370,3 +383,18 @@ def test_a_quantised_layer_behind_another_and_a_selection(box):
     np.testing.assert_array_equal(box.get(outs[1]), ep)
     np.testing.assert_array_equal(box.get(outs[2]), et)
     np.testing.assert_array_equal(box.get(xv).reshape(g, k, 200), np.take_along_axis(x.reshape(g, k, 200), ep[:, :, None], 1))
+
+
+@pytest.mark.parametrize("v", [40, 700, 9000, 70000])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_select_sums_over_wide_ranges(box, v, dtype):
+    """logits that rise by more than an exponential holds, in either direction, and lie far from zero; sums of equal terms"""
+    r = np.random.default_rng(v)
+    up = np.sort(r.normal(size=(1, 2, v)) * 2000, axis=2)
+    sc = -r.random((1, 2))
+    for x in (up, up[:, :, ::-1], up * 1e30 if dtype == "float32" else up * 100, r.normal(size=(1, 2, v)) - 5000, r.normal(size=(1, 2, v)) * 0.01 + 900,
+              np.zeros((1, 2, v)), np.where(np.arange(v) < v // 2, -700.0, 3.0) * np.ones((1, 2, 1))):
+        mask = r.random((1, 2, v)) < 0.5
+        mask[0, 0, -1] = mask[0, 0, 0] = True
+        select_case(box, x, sc, 4, dtype)
+        select_case(box, x, sc, 4, dtype, mask=mask)

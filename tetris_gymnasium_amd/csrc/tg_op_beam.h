@@ -19,10 +19,10 @@ struct SelectArgs {
   int k, v, beams, pad, norm;
 };
 
-// e^d for d <= 0 (or NaN: e^-700; the callers look for NaN themselves) to 1.1e-12 of its value, in 16 instructions: d log2(e) = n + f,
+// e^d for d <= 700 (NaN: e^-700; the callers look for NaN themselves) to 1.1e-12 of its value, in 16 instructions: d log2(e) = n + f,
 // |f| <= 1/2; 2^f is the Chebyshev interpolation of degree 8 on [-1/2, 1/2], and n is added to its exponent.  Below -700 it stays at
 // 1e-304, which is nothing beside the largest term's 1.
-__device__ __forceinline__ double exp_neg(double d) {
+__device__ __forceinline__ double exp64(double d) {
   const double big = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the nearest integer
   const double t = fmax(d, -700.0) * 1.4426950408889634, z = t + big, f = t - (z - big);
   double p = 0x1.63d1279ae38e4p-20;
@@ -36,6 +36,16 @@ __device__ __forceinline__ double exp_neg(double d) {
   p = fma(p, f, 1.0);
   const uint64_t u = (uint64_t)__double_as_longlong(p);
   return __longlong_as_double((long long)(u + ((uint64_t)(uint32_t)(uint64_t)__double_as_longlong(z) << 52)));
+}
+
+// ln(s) for positive normal s: the hardware's float32 logarithm y, then one step of Newton's method to the third order in what it lacks
+// (s e^-y = 1 + z, |z| < 2^-16: z - z^2/2 leaves z^3/3 < 2e-15); the error is that of exp64.
+__device__ __forceinline__ double log64(double s) {
+  int e;
+  const double h = frexp(s, &e);  // (a sum of up to 2^20 terms, but of any magnitude where it is rescaled)
+  const double y = (double)(__builtin_amdgcn_logf((float)h) * 0.693147180559945f);
+  const double z = fma(h, exp64(-y), -1.0);
+  return fma((double)e, 0x1.62e42fefa39efp-1, y + fma(-0.5 * z, z, z));
 }
 
 // A candidate as two words, larger = better, {0, .} = none: the score, then (beam, logit, entry) — within a beam the score never falls
@@ -82,19 +92,24 @@ template <class T> __device__ __forceinline__ T wave_bound(T m, int beams, T (*l
   return group_reduce<64>(larger < beams ? m : top, [](T a, T b) { return a < b ? a : b; });
 }
 
+// A candidate before it is ranked: its score (-inf or NaN: none), its logit, and its beam and entry (row << 24 | entry).
+struct Cand { double c; float x; uint32_t at; };
+__device__ __forceinline__ Key key_of(const Cand& a) { return make_key(a.c, (int)(a.at >> 24), order_f32(a.x), (int)(a.at & 0xFFFFFF)); }
+
 // Of N candidates per lane the best `beams` of the wave, handed to put(rank, key) in descending order; returns how many there are.
 // The bound is taken over the scores rounded to float32 (rounding keeps their order, so nothing that belongs to the best is lost);
-// what reaches it is packed into one candidate per lane through LDS (64 keys per wave) and ranked by counting; where more than 64
-// reach it (many equal ones, many beams), the best is taken out `beams` times instead.
-template <int N, class F> __device__ __forceinline__ int wave_top(Key (&k)[N], int beams, Key* lds, F put) {
+// what reaches it is packed into one candidate per lane through LDS (64 per wave) and ranked by counting; where more than 64 reach it
+// (many equal ones, many beams), the best is taken out `beams` times instead.
+template <int N, class F> __device__ __forceinline__ int wave_top(const Cand (&k)[N], int beams, Cand* lds, F put) {
   const int lane = threadIdx.x & 63;
+  constexpr float low = -3.402823466e38f;  // (a score below the float range is still one)
   float c[N], m = -__builtin_inff();
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    c[i] = k[i].s ? fmaxf((float)unorder_f64(k[i].s), -3.402823466e38f) : -__builtin_inff();  // (a score below the float range is still one)
+    c[i] = k[i].c > -__builtin_inf() ? fmaxf((float)k[i].c, low) : -__builtin_inff();
     m = fmaxf(m, c[i]);
   }
-  const float bound = fmaxf(wave_bound<float>(m, beams, lane_f32, __builtin_inff()), -3.402823466e38f);
+  const float bound = fmaxf(wave_bound<float>(m, beams, lane_f32, __builtin_inff()), low);
   int n = 0, at[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -108,29 +123,35 @@ template <int N, class F> __device__ __forceinline__ int wave_top(Key (&k)[N], i
       if (c[i] >= bound) lds[at[i]] = k[i];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    Key c = {0, 0};
-    if (lane < n) c = lds[lane];
-    int rank = 0;
+    Key key = {0, 0};
+    if (lane < n) key = key_of(lds[lane]);
+    int rank = 0, same = 0;
     for (int l = 0; l < n; ++l) {
-      const Key o = {lane_u64(c.s, l), lane_u64(c.r, l)};
-      rank += better(o, c);
+      const uint64_t o = lane_u64(key.s, l);
+      rank += o > key.s;
+      same += o == key.s;
     }
-    if (lane < n && rank < beams) put(rank, c);
+    if (__ballot(lane < n && same > 1))  // equal scores: by what is behind them
+      for (int l = 0; l < n; ++l) rank += lane_u64(key.s, l) == key.s && lane_u64(key.r, l) > key.r;
+    if (lane < n && rank < beams) put(rank, key);
     __builtin_amdgcn_wave_barrier();
     return n < beams ? n : beams;
   }
+  Key all[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) all[i] = key_of(k[i]);
   for (int b = 0; b < beams; ++b) {
-    Key c = {0, 0};
+    Key best = {0, 0};
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (better(k[i], c)) c = k[i];
-    const uint64_t s = group_reduce<64>(c.s, max_u64), r = group_reduce<64>(c.s == s ? c.r : (uint64_t)0, max_u64);
+      if (better(all[i], best)) best = all[i];
+    const uint64_t s = group_reduce<64>(best.s, max_u64), r = group_reduce<64>(best.s == s ? best.r : (uint64_t)0, max_u64);
     if (s == 0) return b;
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (k[i].s == s && k[i].r == r) {
-        put(b, k[i]);
-        k[i].s = 0;
+      if (all[i].s == s && all[i].r == r) {
+        put(b, all[i]);
+        all[i].s = 0;
       }
   }
   return beams;
@@ -139,7 +160,7 @@ template <int N, class F> __device__ __forceinline__ int wave_top(Key (&k)[N], i
 // Small searches: a wave per group, L = the power of two below 64 / K lanes per beam, N entries per lane (V <= L * N).  The log-sum of
 // a beam is a reduction over its L lanes.  Everything stays in registers; the input is read once.
 template <class T, int N> __global__ __launch_bounds__(256) void select_small_kernel(const SelectArgs a, int shift) {
-  __shared__ Key lds[4][64];
+  __shared__ Cand lds[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t g = (int64_t)blockIdx.x * 4 + wave;
   if (g >= a.groups) return;
@@ -179,7 +200,7 @@ template <class T, int N> __global__ __launch_bounds__(256) void select_small_ke
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       nan |= e[i] != e[i];
-      s += exp_neg((double)e[i] - md);  // (m = -inf: the beam has no candidate, whatever this is)
+      s += exp64((double)e[i] - md);  // (m = -inf: the beam has no candidate, whatever this is)
     }
     if (nan) s = __builtin_nan("");  // (not a distribution: no candidate)
     if (L > 1) s += xor_lane<1>(s);
@@ -188,15 +209,13 @@ template <class T, int N> __global__ __launch_bounds__(256) void select_small_ke
     if (L > 8) s += xor_lane<8>(s);
     if (L > 16) s += xor_lane<16>(s);
     if (L > 32) s += xor_lane<32>(s);
-    lse = md + log(s);
+    lse = md + log64(s);
   }
-  Key k[N];
+  Cand k[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const double c = e[i] > -__builtin_inff() ? (double)sc + ((double)e[i] - lse) : -__builtin_inf();
-    k[i] = make_key(c, jj, order_f32(e[i]), sub + i * L);
-  }
-  if (here && done && sub == 0) k[0] = make_key((double)sc, j, 0, a.pad);
+  for (int i = 0; i < N; ++i)
+    k[i] = {e[i] > -__builtin_inff() ? (double)sc + ((double)e[i] - lse) : -__builtin_inf(), e[i], ((uint32_t)jj << 24) + (uint32_t)(sub + i * L)};
+  if (here && done && sub == 0) k[0] = {(double)sc, 0.0f, ((uint32_t)j << 24) + (uint32_t)a.pad};
   const int64_t o = g * a.beams;
   const int n = wave_top(k, a.beams, lds[wave], [&](int rank, const Key& c) { put_result(a, o + rank, c); });
   if (lane >= n && lane < a.beams) put_result(a, o + lane, Key{0, 0});
@@ -249,24 +268,41 @@ template <class T, int E> __global__ __launch_bounds__(256) void select_chunk_ke
       for (int q = 0; q < V; ++q) e[i * V + q] = v + q < a.v && (!mask || mask[v + q]) ? to_f32(x[v + q]) : -__builtin_inff();
     }
   }
-  float m = -__builtin_inff();
+  // The sum starts as soon as the lane's first entries are there: against their maximum `ref`, not the chunk's (float64 holds e^600 of
+  // it; an entry further above moves the reference), and the lanes' sums are brought to the chunk's maximum at the end.
+  float lm = -__builtin_inff(), ref = 0;
+  double s = 0;
+  bool nan = false;
 #pragma unroll
-  for (int i = 0; i < E; ++i) m = fmaxf(m, e[i]);
-  const float lm = m;  // (of the lane; a NaN is not in it)
-  m = group_reduce<64>(m, [](float p, float q) { return fmaxf(p, q); });
+  for (int i = 0; i < NV; ++i) {
+    float vm = -__builtin_inff();
+#pragma unroll
+    for (int q = 0; q < V; ++q) vm = fmaxf(vm, e[i * V + q]);  // (a NaN is not in it)
+    if (a.norm) {
+      if (lm == -__builtin_inff()) ref = vm > -__builtin_inff() ? vm : 0.0f;
+      const bool far = vm - ref > 600.0f;  // (also where vm is infinite)
+      if (__ballot(far)) {
+        if (far) {
+          s *= exp64((double)ref - (double)vm);
+          ref = vm;
+        }
+      }
+      const double rd = ref;
+#pragma unroll
+      for (int q = 0; q < V; ++q) {
+        nan |= e[i * V + q] != e[i * V + q];
+        s += exp64((double)e[i * V + q] - rd);
+      }
+    }
+    lm = fmaxf(lm, vm);
+  }
+  float m = group_reduce<64>(lm, [](float p, float q) { return fmaxf(p, q); });
   if (lane == 0) wm[wave] = m;
   __syncthreads();
   m = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
-  double s = 0;
   if (a.norm) {
-    bool nan = false;
-#pragma unroll
-    for (int i = 0; i < E; ++i) nan |= e[i] != e[i];
-    const double md = m > -__builtin_inff() ? (double)m : 0.0;  // (nothing allowed: a sum of 0)
-#pragma unroll
-    for (int i = 0; i < E; ++i) s += exp_neg((double)e[i] - md);
+    s = lm > -__builtin_inff() ? s * exp64((double)ref - (double)m) : 0.0;  // (a lane without entries summed e^-700 each)
     if (nan || m == __builtin_inff()) s = __builtin_nan("");
-    if (m == -__builtin_inff()) s = nan ? s : 0.0;
     s = group_reduce<64>(s, [](double p, double q) { return p + q; });
     if (lane == 0) wsum[wave] = s;
   }
@@ -299,67 +335,86 @@ template <class T, int E> __global__ __launch_bounds__(256) void select_chunk_ke
   if (t == 0) *head = {a.norm ? wsum[0] + wsum[1] + wsum[2] + wsum[3] : 0.0, m, keep};
 }
 
-// ... second step: a workgroup per group puts the chunks' sums and lists together.  All heads are read at once, a lane per chunk; the
-// candidates come in rounds of 256, the first entries of all lists before the second ones, so that later rounds soon hold nothing
-// better than the `beams` already found.  A round goes through each of the four waves' own best to the first wave.
+// ... second step: a workgroup per group puts the chunks' sums and lists together.  Candidates come in rounds of 256, the first entries of
+// all lists before the second ones, so that later rounds soon hold nothing better than the `beams` already found; a round goes through
+// each of the four waves' own best to the first wave.  Bound by the latency of its reads: everything the first round needs is asked
+// for at the start.
 __global__ __launch_bounds__(256) void select_merge_kernel(const SelectArgs a, int chunks, const uint8_t* ws) {
-  __shared__ Key lds[4][64], mine[4][64], top[64];
+  __shared__ Cand lds[4][64];
+  __shared__ Key mine[4][64], top[64];
   __shared__ double lse[64];
+  __shared__ float score[64];
   __shared__ int have[4];
   __shared__ Key bottom;  // the worst of the `beams` found so far, or none
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int64_t g = blockIdx.x, pb = select_part_bytes(a.beams);
   const uint8_t* base = ws + g * a.k * chunks * pb;
-  const int lists = a.k * chunks;
-  const int64_t total = (int64_t)lists * a.beams;
-  auto part = [&](int l) { return (const SelectPart*)(base + (int64_t)l * pb); };
-  if (a.norm) {  // a wave per beam, a lane per chunk
-    for (int j = wave; j < a.k; j += 4) {
-      float m = -__builtin_inff();
-      for (int c = lane; c < chunks; c += 64) m = fmaxf(m, part(j * chunks + c)->m);
-      m = group_reduce<64>(m, [](float p, float q) { return fmaxf(p, q); });
-      double s = 0;
-      for (int c = lane; c < chunks; c += 64) {
-        const SelectPart h = *part(j * chunks + c);
-        if (h.s != 0.0) s += h.s * exp_neg((double)h.m - (double)m);
-      }
-      s = group_reduce<64>(s, [](double p, double q) { return p + q; });
-      if (lane == 0) lse[j] = (double)m + log(s);
+  const uint32_t lists = (uint32_t)(a.k * chunks), total = lists * (uint32_t)a.beams;
+  auto part = [&](uint32_t l) { return (const SelectPart*)(base + (int64_t)l * pb); };
+  auto fetch = [&](uint32_t c, uint32_t& row) {  // candidate c of all lists, 0 where its list is shorter
+    uint64_t u = 0;
+    if (c < total) {
+      const uint32_t rank = c / lists, l = c - rank * lists;
+      row = l / (uint32_t)chunks;
+      u = ((const uint64_t*)(part(l) + 1))[rank];
+      if ((int)rank >= part(l)->n) u = 0;
     }
-  } else if (t < a.k) {
+    return u;
+  };
+  uint32_t row = 0;
+  uint64_t u = fetch(t, row);
+  bool done = false;
+  if (t < a.k) {
+    score[t] = a.scores[g * a.k + t];
+    done = a.finished && a.finished[g * a.k + t];
     lse[t] = 0;
   }
   if (t == 0) bottom = {0, 0};
-  int found = 0;
-  for (int64_t i0 = -1; i0 < total; i0 += i0 < 0 ? 1 : 256) {
-    Key k[1] = {{0, 0}};
-    uint64_t u = 0;
-    int row = 0;
-    if (i0 >= 0 && i0 + t < total) {
-      const int64_t c = i0 + t;
-      const int rank = (int)(c / lists), l = (int)(c - (int64_t)rank * lists);
-      row = l / chunks;
-      if (rank < part(l)->n) u = ((const uint64_t*)(part(l) + 1))[rank];
+  if (a.norm) {  // a wave per beam, a lane per chunk
+    __syncthreads();
+    for (int j = wave; j < a.k; j += 4) {
+      float m = -__builtin_inff();
+      double s = 0;
+      for (int c = lane; c < chunks; c += 64) {
+        const SelectPart h = *part((uint32_t)(j * chunks + c));
+        if (h.m > m) {
+          s *= exp64((double)m - (double)h.m);  // (m = -inf: s is 0)
+          m = h.m;
+        }
+        if (h.s != 0.0) s += h.s * exp64((double)h.m - (double)m);
+      }
+      const float all = group_reduce<64>(m, [](float p, float q) { return fmaxf(p, q); });
+      if (s != 0.0) s *= exp64((double)m - (double)all);
+      s = group_reduce<64>(s, [](double p, double q) { return p + q; });
+      if (lane == 0) lse[j] = (double)all + log64(s);
     }
+  }
+  int found = 0;
+  for (uint32_t i0 = 0; i0 < total || i0 == 0; i0 += 256) {
+    if (i0) u = fetch(i0 + t, row);
     __syncthreads();  // (lse; the round before)
+    Cand k[2] = {{-__builtin_inf(), 0.0f, 0}, {-__builtin_inf(), 0.0f, 0}};
     if (u) {
       const float x = unorder_f32((uint32_t)(u >> 32));
-      k[0] = make_key((double)a.scores[g * a.k + row] + ((double)x - lse[row]), row, (uint32_t)(u >> 32), (int)~(uint32_t)u);
-    } else if (i0 < 0 && t < a.k && a.finished && a.finished[g * a.k + t]) {  // first the finished beams, a candidate each
-      k[0] = make_key((double)a.scores[g * a.k + t], t, 0, a.pad);
+      k[0] = {(double)score[row] + ((double)x - lse[row]), x, (row << 24) | ~(uint32_t)u};
+      if (!better(key_of(k[0]), bottom)) k[0].c = -__builtin_inf();
     }
-    if (!better(k[0], bottom)) k[0].s = 0;
+    if (i0 == 0 && done) k[1] = {(double)score[t], 0.0f, ((uint32_t)t << 24) | (uint32_t)a.pad};  // a finished beam's one candidate
     int n = 0;
-    if (__ballot(k[0].s != 0)) {
+    if (__ballot(k[0].c > -__builtin_inf() || k[1].c > -__builtin_inf()))
       n = wave_top(k, a.beams, lds[wave], [&](int rank, const Key& c) { mine[wave][rank] = c; });
-    }
     if (lane == 0) have[wave] = n;
     __syncthreads();
     if (wave == 0 && have[0] + have[1] + have[2] + have[3] > 0) {
-      Key all[5];
+      Cand all[5];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) all[i] = lane < have[i] ? mine[i][lane] : Key{0, 0};
-      all[4] = lane < found ? top[lane] : Key{0, 0};
+      for (int i = 0; i < 5; ++i) {
+        Key c = {0, 0};
+        if (i < 4) { if (lane < have[i]) c = mine[i][lane]; }
+        else if (lane < found) c = top[lane];
+        all[i] = {c.s ? unorder_f64(c.s) : -__builtin_inf(), unorder_f32((uint32_t)(c.r >> 24)),
+                  ((uint32_t)(63 - (int)(c.r >> 56)) << 24) | (uint32_t)(0xFFFFFF - (c.r & 0xFFFFFF))};
+      }
       __builtin_amdgcn_wave_barrier();
       found = wave_top(all, a.beams, lds[0], [&](int rank, const Key& c) { top[rank] = c; });
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

@@ -69,12 +69,13 @@ constexpr int kUnits = 256;  // compute units
 
 template <class OT, bool U8, int KS> void linear_rows(const LinearArgs& a, hipStream_t st) {
   const int64_t cols = (a.n + 63) / 64;
-  const int strips = cols >= 4 ? 4 : cols == 2 ? 2 : 1, below = 4 / strips;
-  const int64_t gy = (cols + strips - 1) / strips, tiles = (a.rows + 15) / 16;
+  const int shift = cols >= 4 ? 2 : cols == 2 ? 1 : 0, below = 4 >> shift;
+  const int64_t gy = (cols + (1 << shift) - 1) >> shift, tiles = (a.rows + 15) / 16;
   // as many workgroups as stay resident (by the variant's registers), each with a run of tiles
-  int64_t gx = (kUnits * (KS == 1 ? 3 : 2) + gy - 1) / gy;
+  int64_t gx = (kUnits * (KS == 1 ? 4 : 2) + gy - 1) / gy;
   if (gx > (tiles + below - 1) / below) gx = (tiles + below - 1) / below;
-  hipLaunchKernelGGL((linear_rows_kernel<OT, U8, KS>), dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, st, a, strips);
+  const int64_t inside = a.x_stride ? ((a.rows - 1) * a.x_stride + a.k - 64 * KS) / (16 * a.x_stride) : 0;
+  hipLaunchKernelGGL((linear_rows_kernel<OT, U8, KS>), dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, st, a, shift, inside);
 }
 
 template <class OT, bool U8, int T, int U> void linear_few(const LinearArgs& a, hipStream_t st) {
@@ -99,20 +100,31 @@ template <class OT, bool U8, int BM, int BN, int WM, int WN, bool AL> void linea
   }
 }
 
+// Times in us, back to back, bf16 out; rows x k x n.
 template <class OT, bool U8> void linear_launch(const LinearArgs& a, hipStream_t st) {
-  if (a.rows <= 64) {
-    if (a.rows <= 16) return linear_few<OT, U8, 1, 1>(a, st);
-    if (a.rows <= 32) return linear_few<OT, U8, 2, 2>(a, st);
-    return linear_few<OT, U8, 2, 4>(a, st);
+  const auto tiles = [&](int64_t bm, int64_t bn) { return ((a.rows + bm - 1) / bm) * ((a.n + bn - 1) / bn); };
+  // Few rows: the waves of a workgroup share K.  The widest variant that still gives every compute unit a workgroup: 64 x 4 096 x 8 192:
+  // 15.3 (2, 4) against 17.7 (2, 2) and 30.7 (1, 1), but 64 x 1 024 x 1 024: 6.7, 4.8, 3.4.  Above 64 rows only where tiles would leave
+  // most of the units idle: 128 x 1 024 x 1 024: 4.2 against 6.2; 128 x 4 096 x 8 192: 25.5 against 19.8.
+  if (a.rows <= 64 || (a.rows <= 256 && tiles(64, 64) <= 64)) {
+    if (a.rows > 32 && tiles(64, 32) >= kUnits) return linear_few<OT, U8, 2, 4>(a, st);
+    if (a.rows > 16 && tiles(32, 32) >= kUnits) return linear_few<OT, U8, 2, 2>(a, st);
+    if (tiles(16, 32) >= kUnits) return linear_few<OT, U8, 2, 1>(a, st);
+    return linear_few<OT, U8, 1, 1>(a, st);
   }
+  // Short rows: weights in registers.  Rows at 16-byte addresses are better off in tiles from 128 bytes on: 65 536 x 256 x 40: 7.6 against
+  // 9.5, x 256: 18.4 against 19.8; 65 536 x 200 x 256, whose rows are not: 17.1 against 21.2.
+  const bool al = (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.x_stride | (uintptr_t)a.w_stride | (uintptr_t)a.k) & 15) == 0;
   if (a.k <= 64) return linear_rows<OT, U8, 1>(a, st);
   if (a.k <= 128) return linear_rows<OT, U8, 2>(a, st);
-  if (a.k <= 256) return linear_rows<OT, U8, 4>(a, st);
-  const bool al = (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.x_stride | (uintptr_t)a.w_stride | (uintptr_t)a.k) & 15) == 0;
-  const int64_t big = ((a.rows + 255) / 256) * ((a.n + 255) / 256);
+  if (a.k <= 256 && !al) return linear_rows<OT, U8, 4>(a, st);
+  // Tiles.  4 096 x 4 096 x 4 096 (256 of 256 x 256): 66 against 79 (128 x 128); 2 048 x 4 096 x 4 096 (128; 512 of 128 x 128): 52, 42, 53
+  // (128 x 64); 1 024 x 4 096 x 4 096 (512 of 128 x 64): 29 (128 x 128), 27, 30 (64 x 64); 256 x 4 096 x 4 096: 19 (128 x 64), 15 (64 x 64).
   if (!al) return linear_tile<OT, U8, 128, 128, 2, 2, false>(a, st);
-  if (big >= kUnits) return linear_tile<OT, U8, 256, 256, 2, 4, true>(a, st);
-  return linear_tile<OT, U8, 128, 128, 2, 2, true>(a, st);
+  if (a.n > 128 && a.k >= 512 && tiles(256, 256) >= kUnits) return linear_tile<OT, U8, 256, 256, 2, 4, true>(a, st);
+  if (a.n > 64 && tiles(128, 128) >= 2 * kUnits) return linear_tile<OT, U8, 128, 128, 2, 2, true>(a, st);
+  if (tiles(128, 64) >= 2 * kUnits) return linear_tile<OT, U8, 128, 64, 2, 2, true>(a, st);
+  return linear_tile<OT, U8, 64, 64, 2, 2, true>(a, st);
 }
 
 }  // namespace
