@@ -124,15 +124,22 @@ template <int N, class F> __device__ __forceinline__ int wave_top(const Cand (&k
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     Key key = {0, 0};
-    if (lane < n) key = key_of(lds[lane]);
+    float f = -__builtin_inff();
+    if (lane < n) {
+      const Cand o = lds[lane];
+      key = key_of(o);
+      f = (float)o.c;
+    }
     int rank = 0, same = 0;
     for (int l = 0; l < n; ++l) {
-      const uint64_t o = lane_u64(key.s, l);
-      rank += o > key.s;
-      same += o == key.s;
+      const float o = lane_f32(f, l);
+      rank += o > f;
+      same += o == f;
     }
-    if (__ballot(lane < n && same > 1))  // equal scores: by what is behind them
-      for (int l = 0; l < n; ++l) rank += lane_u64(key.s, l) == key.s && lane_u64(key.r, l) > key.r;
+    if (__ballot(lane < n && same > 1)) {  // equal in float32: by the whole key
+      rank = 0;
+      for (int l = 0; l < n; ++l) rank += better(Key{lane_u64(key.s, l), lane_u64(key.r, l)}, key);
+    }
     if (lane < n && rank < beams) put(rank, key);
     __builtin_amdgcn_wave_barrier();
     return n < beams ? n : beams;
@@ -243,10 +250,8 @@ template <class T, int E> __global__ __launch_bounds__(256) void select_chunk_ke
   uint8_t* part = ws + (int64_t)blockIdx.x * select_part_bytes(a.beams);
   SelectPart* head = (SelectPart*)part;
   uint64_t* keys = (uint64_t*)(part + 16);
-  if ((a.finished && a.finished[row]) || !(a.scores[row] > -__builtin_inff())) {  // (offers nothing of its own)
-    if (t == 0) *head = {0.0, -__builtin_inff(), 0};
-    return;
-  }
+  const float score = a.scores[row];
+  const uint8_t done = a.finished ? a.finished[row] : 0;
   if (t == 0) count = 0;
   const T* x = (const T*)a.x + g * a.lg + j * a.lk;
   const uint8_t* mask = a.mask ? a.mask + g * a.mg + j * a.mk : nullptr;
@@ -267,6 +272,10 @@ template <class T, int E> __global__ __launch_bounds__(256) void select_chunk_ke
 #pragma unroll
       for (int q = 0; q < V; ++q) e[i * V + q] = v + q < a.v && (!mask || mask[v + q]) ? to_f32(x[v + q]) : -__builtin_inff();
     }
+  }
+  if (done || !(score > -__builtin_inff())) {  // (offers nothing of its own; asked behind the loads, not in front of them)
+    if (t == 0) *head = {0.0, -__builtin_inff(), 0};
+    return;
   }
   // The sum starts as soon as the lane's first entries are there: against their maximum `ref`, not the chunk's (float64 holds e^600 of
   // it; an entry further above moves the reference), and the lanes' sums are brought to the chunk's maximum at the end.
@@ -306,22 +315,36 @@ template <class T, int E> __global__ __launch_bounds__(256) void select_chunk_ke
     s = group_reduce<64>(s, [](double p, double q) { return p + q; });
     if (lane == 0) wsum[wave] = s;
   }
-  // the lane's best entry, the wave's bound, and what reaches it
-  int best = 0;
-  float bx = -__builtin_inff();
-#pragma unroll
-  for (int i = E - 1; i >= 0; --i)
-    if (e[i] == lm && lm > -__builtin_inff()) { best = i; bx = lm; }
+  // What reaches the wave's bound is listed.  The bound goes by the logit alone first; only where equal logits bring more than the list
+  // holds, it is drawn again over (logit, place), which are all different.
   auto entry = [&](int i) { return v0 + (i / V) * 256 * V + i % V; };
-  auto key = [&](float f, int v) { return f > -__builtin_inff() ? ((uint64_t)order_f32(f) << 32) | (uint32_t)~v : 0ull; };
-  const uint64_t bound = wave_bound<uint64_t>(key(bx, entry(best)), a.beams, lane_u64, ~(uint64_t)0);
-  const float bf = bound ? unorder_f32((uint32_t)(bound >> 32)) : -3.402823466e38f;
+  auto key = [&](float f, int v) { return ((uint64_t)order_f32(f) << 32) | (uint32_t)~v; };
+  const int room = select_list(a.beams, E);
+  const float bf = fmaxf(wave_bound<float>(lm, a.beams, lane_f32, __builtin_inff()), -3.402823466e38f);
 #pragma unroll
   for (int i = 0; i < E; ++i) {
-    const bool maybe = e[i] >= bf;
-    if (__ballot(maybe)) {
-      const uint64_t k = maybe ? key(e[i], entry(i)) : 0;
-      if (k && k >= bound) list[atomicAdd(&count, 1)] = k;
+    const bool in = e[i] >= bf;
+    if (__ballot(in)) {
+      if (in) {
+        const int at = atomicAdd(&count, 1);
+        if (at < room) list[at] = key(e[i], entry(i));
+      }
+    }
+  }
+  __syncthreads();
+  if (count > room) {
+    __syncthreads();
+    if (t == 0) count = 0;
+    __syncthreads();
+    uint64_t best = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (e[i] > -__builtin_inff()) best = max_u64(best, key(e[i], entry(i)));
+    const uint64_t bound = max_u64(wave_bound<uint64_t>(best, a.beams, lane_u64, ~(uint64_t)0), 1);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const uint64_t k = e[i] > -__builtin_inff() ? key(e[i], entry(i)) : 0;
+      if (k >= bound) list[atomicAdd(&count, 1)] = k;
     }
   }
   __syncthreads();
@@ -335,43 +358,46 @@ template <class T, int E> __global__ __launch_bounds__(256) void select_chunk_ke
   if (t == 0) *head = {a.norm ? wsum[0] + wsum[1] + wsum[2] + wsum[3] : 0.0, m, keep};
 }
 
-// ... second step: a workgroup per group puts the chunks' sums and lists together.  Candidates come in rounds of 256, the first entries of
-// all lists before the second ones, so that later rounds soon hold nothing better than the `beams` already found; a round goes through
-// each of the four waves' own best to the first wave.  Bound by the latency of its reads: everything the first round needs is asked
-// for at the start.
+// ... second step: a workgroup per group puts the chunks' sums together, a wave per beam and a lane per chunk; its first wave then goes
+// through the candidates in rounds of 256, the first entries of all lists before the second ones, so that later rounds soon hold
+// nothing better than the `beams` already found.  Bound by latency (one small workgroup per group): the first round's candidates are
+// asked for at the start.
 __global__ __launch_bounds__(256) void select_merge_kernel(const SelectArgs a, int chunks, const uint8_t* ws) {
-  __shared__ Cand lds[4][64];
-  __shared__ Key mine[4][64], top[64];
+  constexpr int N = 4;
+  __shared__ Cand lds[64];
+  __shared__ Key top[64];
   __shared__ double lse[64];
   __shared__ float score[64];
-  __shared__ int have[4];
-  __shared__ Key bottom;  // the worst of the `beams` found so far, or none
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int64_t g = blockIdx.x, pb = select_part_bytes(a.beams);
   const uint8_t* base = ws + g * a.k * chunks * pb;
   const uint32_t lists = (uint32_t)(a.k * chunks), total = lists * (uint32_t)a.beams;
   auto part = [&](uint32_t l) { return (const SelectPart*)(base + (int64_t)l * pb); };
-  auto fetch = [&](uint32_t c, uint32_t& row) {  // candidate c of all lists, 0 where its list is shorter
-    uint64_t u = 0;
-    if (c < total) {
-      const uint32_t rank = c / lists, l = c - rank * lists;
-      row = l / (uint32_t)chunks;
-      u = ((const uint64_t*)(part(l) + 1))[rank];
-      if ((int)rank >= part(l)->n) u = 0;
+  uint64_t u[N];
+  uint32_t row[N];
+  auto fetch = [&](uint32_t c0) {  // candidates of all lists, 0 where a list is shorter
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t c = c0 + 64 * i + lane;
+      u[i] = row[i] = 0;
+      if (c < total) {
+        const uint32_t rank = c / lists, l = c - rank * lists;
+        row[i] = l / (uint32_t)chunks;
+        u[i] = ((const uint64_t*)(part(l) + 1))[rank];
+        if ((int)rank >= part(l)->n) u[i] = 0;
+      }
     }
-    return u;
   };
-  uint32_t row = 0;
-  uint64_t u = fetch(t, row);
   bool done = false;
-  if (t < a.k) {
-    score[t] = a.scores[g * a.k + t];
-    done = a.finished && a.finished[g * a.k + t];
-    lse[t] = 0;
+  if (wave == 0) {
+    fetch(0);
+    if (lane < a.k) {
+      score[lane] = a.scores[g * a.k + lane];
+      done = a.finished && a.finished[g * a.k + lane];
+      if (!a.norm) lse[lane] = 0;
+    }
   }
-  if (t == 0) bottom = {0, 0};
-  if (a.norm) {  // a wave per beam, a lane per chunk
-    __syncthreads();
+  if (a.norm) {
     for (int j = wave; j < a.k; j += 4) {
       float m = -__builtin_inff();
       double s = 0;
@@ -389,40 +415,41 @@ __global__ __launch_bounds__(256) void select_merge_kernel(const SelectArgs a, i
       if (lane == 0) lse[j] = (double)all + log64(s);
     }
   }
+  __syncthreads();
+  if (wave) return;
   int found = 0;
-  for (uint32_t i0 = 0; i0 < total || i0 == 0; i0 += 256) {
-    if (i0) u = fetch(i0 + t, row);
-    __syncthreads();  // (lse; the round before)
-    Cand k[2] = {{-__builtin_inf(), 0.0f, 0}, {-__builtin_inf(), 0.0f, 0}};
-    if (u) {
-      const float x = unorder_f32((uint32_t)(u >> 32));
-      k[0] = {(double)score[row] + ((double)x - lse[row]), x, (row << 24) | ~(uint32_t)u};
-      if (!better(key_of(k[0]), bottom)) k[0].c = -__builtin_inf();
-    }
-    if (i0 == 0 && done) k[1] = {(double)score[t], 0.0f, ((uint32_t)t << 24) | (uint32_t)a.pad};  // a finished beam's one candidate
-    int n = 0;
-    if (__ballot(k[0].c > -__builtin_inf() || k[1].c > -__builtin_inf()))
-      n = wave_top(k, a.beams, lds[wave], [&](int rank, const Key& c) { mine[wave][rank] = c; });
-    if (lane == 0) have[wave] = n;
-    __syncthreads();
-    if (wave == 0 && have[0] + have[1] + have[2] + have[3] > 0) {
-      Cand all[5];
+  Key bottom = {0, 0};  // the worst of the `beams` found so far, or none
+  for (uint32_t i0 = 0;; i0 += 64 * N) {
+    Cand k[N + 1];
+    bool any = false;
 #pragma unroll
-      for (int i = 0; i < 5; ++i) {
-        Key c = {0, 0};
-        if (i < 4) { if (lane < have[i]) c = mine[i][lane]; }
-        else if (lane < found) c = top[lane];
-        all[i] = {c.s ? unorder_f64(c.s) : -__builtin_inf(), unorder_f32((uint32_t)(c.r >> 24)),
-                  ((uint32_t)(63 - (int)(c.r >> 56)) << 24) | (uint32_t)(0xFFFFFF - (c.r & 0xFFFFFF))};
-      }
+    for (int i = 0; i < N; ++i) {
+      const float x = unorder_f32((uint32_t)(u[i] >> 32));
+      k[i] = {u[i] ? (double)score[row[i]] + ((double)x - lse[row[i]]) : -__builtin_inf(), x, (row[i] << 24) | ~(uint32_t)u[i]};
+      if (found == a.beams && !better(key_of(k[i]), bottom)) k[i].c = -__builtin_inf();
+      any |= k[i].c > -__builtin_inf();
+    }
+    // behind them a finished beam's one candidate, or what was found before
+    k[N] = {-__builtin_inf(), 0.0f, 0};
+    if (i0 == 0) {
+      if (done) k[N] = {(double)score[lane], 0.0f, ((uint32_t)lane << 24) | (uint32_t)a.pad};
+      any |= done;
+    } else if (lane < found) {
+      const Key c = top[lane];
+      k[N] = {unorder_f64(c.s), unorder_f32((uint32_t)(c.r >> 24)), ((uint32_t)(63 - (int)(c.r >> 56)) << 24) | (uint32_t)(0xFFFFFF - (c.r & 0xFFFFFF))};
+    }
+    const bool more = i0 + 64 * N < total;
+    if (more) fetch(i0 + 64 * N);
+    if (__ballot(any)) {
       __builtin_amdgcn_wave_barrier();
-      found = wave_top(all, a.beams, lds[0], [&](int rank, const Key& c) { top[rank] = c; });
+      found = wave_top(k, a.beams, lds, [&](int rank, const Key& c) { top[rank] = c; });
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
-      if (found == a.beams && lane == 0) bottom = top[a.beams - 1];
+      if (found == a.beams) bottom = top[a.beams - 1];
     }
+    if (!more) break;
   }
-  if (t < a.beams) put_result(a, g * a.beams + t, t < found ? top[t] : Key{0, 0});  // (wave 0: beams <= 64)
+  if (lane < a.beams) put_result(a, g * a.beams + lane, lane < found ? top[lane] : Key{0, 0});
 }
 
 // which of them, by sizes alone (the workspace goes by it)
