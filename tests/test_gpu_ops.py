@@ -149,7 +149,7 @@ def quantize_case(box, x, dtype, pitch=None, before=0, qpitch=None):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
-@pytest.mark.parametrize("rows,k", [(1, 1), (3, 7), (17, 40), (5, 256), (33, 257), (4, 512), (2, 1000), (9, 1025), (3, 2048), (2, 4100), (2, 8192), (1, 20011)])
+@pytest.mark.parametrize("rows,k", [(1, 1), (3, 7), (17, 40), (5, 256), (33, 257), (4, 512), (2, 1000), (9, 1025), (3, 2048), (2, 4100), (2, 8192), (1, 20011), (70, 16), (65, 31), (64, 64), (3, 16384), (2, 16500)])
 def test_quantize_sizes(box, rows, k, dtype):
     r = np.random.default_rng(rows * k)
     x = r.normal(size=(rows, k)) * np.exp(2 * r.normal(size=(rows, 1)))

@@ -116,9 +116,11 @@ template <class T, int LPR, int NV> __global__ __launch_bounds__(256) void quant
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int64_t k = ((int64_t)i * LPR + l) * V;
-    h[i] = q_load(xr, k < K ? k : K, K);
-    top = q_top<T>(h[i], top);
+    if (k < K) h[i] = q_load(xr, k, K);
+    else h[i] = QVec<T>{};
   }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) top = q_top<T>(h[i], top);
   for (int64_t k = ((int64_t)NV * LPR + l) * V; k < K; k += LPR * V) top = q_top<T>(q_load(xr, k, K), top);
   top = group_reduce<(LPR < 64 ? LPR : 64)>(top, q_top_join<T>);
   if constexpr (LPR > 64) {

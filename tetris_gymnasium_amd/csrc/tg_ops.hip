@@ -187,13 +187,24 @@ int tg_quantize_i8(int device, void* stream, const void* x, int x_type, int64_t 
     using T = decltype(e);
     const int64_t vec = kQVec<T>;
     const auto grid = [&](int rpb) { return dim3((unsigned)((rows + rpb - 1) / rpb)); };
-    if (k <= 16 * 4 * vec) hipLaunchKernelGGL((quantize_kernel<T, 16, 4>), grid(16), dim3(256), 0, (hipStream_t)stream, (const T*)x, rows, k, x_stride, q, q_stride, scale);
-    else if (k <= 64 * 4 * vec) hipLaunchKernelGGL((quantize_kernel<T, 64, 4>), grid(4), dim3(256), 0, (hipStream_t)stream, (const T*)x, rows, k, x_stride, q, q_stride, scale);
+    const auto run = [&](auto kernel, int rpb) { hipLaunchKernelGGL(kernel, grid(rpb), dim3(256), 0, (hipStream_t)stream, (const T*)x, rows, k, x_stride, q, q_stride, scale); };
+    // rows in as few registers as they need: four or sixteen lanes a row, then a wave, then a workgroup
+    if (k <= 4 * vec) run(quantize_kernel<T, 4, 1>, 64);
+    else if (k <= 8 * vec) run(quantize_kernel<T, 4, 2>, 64);
+    else if (k <= 16 * vec) run(quantize_kernel<T, 16, 1>, 16);
+    else if (k <= 32 * vec) run(quantize_kernel<T, 16, 2>, 16);
+    else if (k <= 64 * vec) run(quantize_kernel<T, 16, 4>, 16);
+    else if (k <= 128 * vec) run(quantize_kernel<T, 64, 2>, 4);
+    else if (k <= 256 * vec) run(quantize_kernel<T, 64, 4>, 4);
     else {
       for (int64_t r = 0; r < rows; r += kMaxGrid) {
         const int64_t c = rows - r < kMaxGrid ? rows - r : kMaxGrid;
-        hipLaunchKernelGGL((quantize_kernel<T, 256, 4>), dim3((unsigned)c), dim3(256), 0, (hipStream_t)stream, (const T*)x + r * x_stride, c, k,
-                           x_stride, q + r * q_stride, q_stride, scale + r);
+        const auto part = [&](auto kernel) {
+          hipLaunchKernelGGL(kernel, dim3((unsigned)c), dim3(256), 0, (hipStream_t)stream, (const T*)x + r * x_stride, c, k, x_stride, q + r * q_stride, q_stride, scale + r);
+        };
+        if (k <= 512 * vec) part(quantize_kernel<T, 256, 2>);
+        else if (k <= 1024 * vec) part(quantize_kernel<T, 256, 4>);
+        else part(quantize_kernel<T, 256, 8>);
       }
     }
     return 0;
