@@ -240,7 +240,8 @@ def select_case(box, x, sc, beams, dtype="float32", mask=None, done=None, pad=0,
 
 
 SIZES = [(1, 1, 1, 1), (1, 4, 40, 4), (3, 1, 5, 3), (5, 8, 40, 8), (2, 3, 7, 16), (4, 16, 128, 16), (2, 64, 9, 64), (3, 2, 300, 64), (1, 8, 1000, 8),
-         (2, 5, 1031, 7), (2, 8, 4097, 8), (1, 3, 8192, 33), (1, 2, 20000, 5), (1, 16, 9001, 64), (70, 8, 40, 8), (300, 2, 8, 3)]
+         (2, 5, 1031, 7), (2, 8, 4097, 8), (1, 3, 8192, 33), (1, 2, 20000, 5), (1, 16, 9001, 64), (70, 8, 40, 8), (300, 2, 8, 3), (64, 8, 9000, 64), (130, 4, 3000, 20), (300, 4, 2000, 7), (20, 64, 17, 3),
+         (9, 33, 129, 40), (1, 1, 1024, 64), (1, 1, 1025, 1)]
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])

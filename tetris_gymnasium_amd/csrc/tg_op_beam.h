@@ -174,21 +174,28 @@ template <class T, int N> __global__ __launch_bounds__(256) void select_small_ke
   const int L = 1 << shift, j = lane >> shift, sub = lane & (L - 1);
   const bool here = j < a.k;
   const int jj = here ? j : 0;
-  const float sc = a.scores[g * a.k + jj];
-  const bool done = a.finished && a.finished[g * a.k + jj];
   const T* x = (const T*)a.x + g * a.lg + jj * a.lk;
-  const uint8_t* mask = a.mask ? a.mask + g * a.mg + jj * a.mk : nullptr;
   T raw[N];
-  uint8_t ok[N];
+  uint32_t at[N], ok[N];  // (every load in front of the first use: a wave waits for memory once)
 #pragma unroll
-  for (int i = 0; i < N; ++i) {  // (all loads first)
-    const int v = sub + i * L, vv = v < a.v ? v : 0;
-    raw[i] = x[vv];
-    ok[i] = mask ? mask[vv] : 1;
+  for (int i = 0; i < N; ++i) {
+    const int v = sub + i * L;
+    at[i] = v < a.v ? v : 0;
+    raw[i] = x[at[i]];
+    ok[i] = 1;
   }
+  const float sc = a.scores[g * a.k + jj];
+  uint32_t fin = 0;
+  if (a.finished) fin = a.finished[g * a.k + jj];
+  if (a.mask) {
+    const uint8_t* mask = a.mask + g * a.mg + jj * a.mk;
+#pragma unroll
+    for (int i = 0; i < N; ++i) ok[i] = mask[at[i]];
+  }
+  const bool done = fin != 0;
   float e[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) e[i] = here && !done && ok[i] && sub + i * L < a.v ? to_f32(raw[i]) : -__builtin_inff();
+  for (int i = 0; i < N; ++i) e[i] = here && !done && ok[i] != 0 && sub + i * L < a.v ? to_f32(raw[i]) : -__builtin_inff();
   double lse = 0;
   if (a.norm) {
     float m = -__builtin_inff();
@@ -254,23 +261,34 @@ template <class T, int E> __global__ __launch_bounds__(256) void select_chunk_ke
   const uint8_t done = a.finished ? a.finished[row] : 0;
   if (t == 0) count = 0;
   const T* x = (const T*)a.x + g * a.lg + j * a.lk;
-  const uint8_t* mask = a.mask ? a.mask + g * a.mg + j * a.mk : nullptr;
+  const uint8_t* mask = a.mask + g * a.mg + j * a.mk;  // (only where a.mask is)
   const int v0 = chunk * (256 * E) + t * V;
   float e[E];
+  if ((chunk + 1) * (256 * E) <= a.v) {  // a whole chunk: every load in front of the first use
+    v4i u[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = v0 + i * 256 * V;
-    if (v + V <= a.v) {
-      const v4i u = load16(x + v);
+    for (int i = 0; i < NV; ++i) u[i] = load16(x + v0 + i * 256 * V);
+    struct __attribute__((packed, aligned(1))) Bytes { uint8_t b[V]; } ok[NV];
+    if (a.mask) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) ok[i] = *(const Bytes*)(mask + v0 + i * 256 * V);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
       T h[V];
-      __builtin_memcpy(h, &u, 16);
-      uint8_t ok[V];
-      if (mask) __builtin_memcpy(ok, mask + v, V);
+      __builtin_memcpy(h, &u[i], 16);
 #pragma unroll
-      for (int q = 0; q < V; ++q) e[i * V + q] = !mask || ok[q] ? to_f32(h[q]) : -__builtin_inff();
-    } else {
+      for (int q = 0; q < V; ++q) e[i * V + q] = to_f32(h[q]);
+    }
+    if (a.mask) {
 #pragma unroll
-      for (int q = 0; q < V; ++q) e[i * V + q] = v + q < a.v && (!mask || mask[v + q]) ? to_f32(x[v + q]) : -__builtin_inff();
+      for (int i = 0; i < E; ++i) e[i] = ok[i / V].b[i % V] ? e[i] : -__builtin_inff();
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int v = v0 + (i / V) * 256 * V + i % V;
+      e[i] = v < a.v && (!a.mask || mask[v]) ? to_f32(x[v]) : -__builtin_inff();
     }
   }
   if (done || !(score > -__builtin_inff())) {  // (offers nothing of its own; asked behind the loads, not in front of them)

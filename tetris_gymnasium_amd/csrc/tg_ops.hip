@@ -72,7 +72,7 @@ template <class OT, bool U8, int KS> void linear_rows(const LinearArgs& a, hipSt
   const int shift = cols >= 4 ? 2 : cols == 2 ? 1 : 0, below = 4 >> shift;
   const int64_t gy = (cols + (1 << shift) - 1) >> shift, tiles = (a.rows + 15) / 16;
   // as many workgroups as stay resident (by the variant's registers), each with a run of tiles
-  int64_t gx = (kUnits * (KS == 1 ? 4 : 2) + gy - 1) / gy;
+  int64_t gx = (kUnits * (KS == 1 ? 3 : 2) + gy - 1) / gy;
   if (gx > (tiles + below - 1) / below) gx = (tiles + below - 1) / below;
   const int64_t inside = a.x_stride ? ((a.rows - 1) * a.x_stride + a.k - 64 * KS) / (16 * a.x_stride) : 0;
   hipLaunchKernelGGL((linear_rows_kernel<OT, U8, KS>), dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, st, a, shift, inside);
@@ -112,12 +112,12 @@ template <class OT, bool U8> void linear_launch(const LinearArgs& a, hipStream_t
     if (tiles(16, 32) >= kUnits) return linear_few<OT, U8, 2, 1>(a, st);
     return linear_few<OT, U8, 1, 1>(a, st);
   }
-  // Short rows: weights in registers.  Rows at 16-byte addresses are better off in tiles from 128 bytes on: 65 536 x 256 x 40: 7.6 against
-  // 9.5, x 256: 18.4 against 19.8; 65 536 x 200 x 256, whose rows are not: 17.1 against 21.2.
+  // Short rows: weights in registers: 65 536 x 200 x 256: 16.1 against 20.9 (tiles), x 256 x 256: 17.1 against 18.1; only where they would
+  // multiply mostly columns that are not there, and 16-byte addresses allow it, tiles are better: x 256 x 40: 8.3 against 7.6.
   const bool al = (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.x_stride | (uintptr_t)a.w_stride | (uintptr_t)a.k) & 15) == 0;
   if (a.k <= 64) return linear_rows<OT, U8, 1>(a, st);
   if (a.k <= 128) return linear_rows<OT, U8, 2>(a, st);
-  if (a.k <= 256 && !al) return linear_rows<OT, U8, 4>(a, st);
+  if (a.k <= 256 && !(al && a.n <= 64)) return linear_rows<OT, U8, 4>(a, st);
   // Tiles.  4 096 x 4 096 x 4 096 (256 of 256 x 256): 66 against 79 (128 x 128); 2 048 x 4 096 x 4 096 (128; 512 of 128 x 128): 52, 42, 53
   // (128 x 64); 1 024 x 4 096 x 4 096 (512 of 128 x 64): 29 (128 x 128), 27, 30 (64 x 64); 256 x 4 096 x 4 096: 19 (128 x 64), 15 (64 x 64).
   if (!al) return linear_tile<OT, U8, 128, 128, 2, 2, false>(a, st);
