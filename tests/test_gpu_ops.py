@@ -234,9 +234,9 @@ def select_case(box, x, sc, beams, dtype="float32", mask=None, done=None, pad=0,
     gs, gp, gt = (box.get(o) for o in outs)
     np.testing.assert_array_equal(gp, ep)
     np.testing.assert_array_equal(gt, et)
-    same = es == gs
+    same = es == gs  # (-inf on both sides too)
     # one rounding to float32 of a score held in 64 bits (its log-sum to 1e-12)
-    assert (same | (np.abs(gs - es) <= np.abs(np.where(same, 0, es)) * 2.0**-24 * 1.001 + 1e-11)).all()
+    assert (same | (np.abs(np.where(same, 0, gs) - np.where(same, 0, es)) <= np.abs(np.where(same, 0, es)) * 2.0**-24 * 1.001 + 1e-11)).all()
 
 
 SIZES = [(1, 1, 1, 1), (1, 4, 40, 4), (3, 1, 5, 3), (5, 8, 40, 8), (2, 3, 7, 16), (4, 16, 128, 16), (2, 64, 9, 64), (3, 2, 300, 64), (1, 8, 1000, 8),
@@ -311,7 +311,8 @@ def test_select_strides(box):
 
 # ---- beam_reorder ---------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("g,kin,kout", [(1, 1, 1), (3, 4, 4), (2, 8, 8), (5, 3, 7), (4, 16, 2), (1, 64, 64), (33, 2, 2)])
-@pytest.mark.parametrize("rows", [(200, 40, 32, 48), (1,), (13, 7, 3), (4096, 36), (1000, 2), (16, 24, 4, 8, 6)])
+@pytest.mark.parametrize("rows", [(200, 40, 32, 48), (1,), (13, 7, 3), (4096, 36), (1000, 2), (16, 24, 4, 8, 6), (17, 31, 33, 5001),
+                                  tuple(range(5, 29))])
 def test_reorder(box, g, kin, kout, rows):
     r = np.random.default_rng(g + kin * 10 + len(rows))
     src = [r.integers(0, 256, (g * kin, n)).astype(np.uint8) for n in rows]

@@ -104,8 +104,11 @@ def linear_scorer(w, seed):
     return PlacementScorer([(r.integers(-20, 8, (1, w + 3)).astype(np.int8), np.array([2.0**-6], np.float32), np.array([0.5], np.float32))])
 
 
-@pytest.mark.parametrize("w,h,G,K,depth,warm", [(10, 20, 5, 4, 5, 0), (6, 12, 7, 8, 12, 9), (10, 20, 3, 1, 3, 4), (10, 24, 2, 16, 6, 20)])
-def test_plan_is_the_search_done_on_the_host(w, h, G, K, depth, warm):
+@pytest.mark.parametrize("w,h,G,K,depth,warm,packed", [(10, 20, 5, 4, 5, 0, 0), (6, 12, 7, 8, 12, 9, 0), (10, 20, 3, 1, 3, 4, 0), (10, 24, 2, 16, 6, 20, 0),
+                                                       (10, 20, 4, 6, 8, 11, 1)])
+def test_plan_is_the_search_done_on_the_host(w, h, G, K, depth, warm, packed, monkeypatch):
+    if packed:  # nibble boards
+        monkeypatch.setenv("TG_PACKED", "1")
     main = Engine(G, w, h, obs_mode=N.OBS_BOARD, grouped=True)
     main.reset(np.arange(5, 5 + G, dtype=np.uint64))
     for t in range(warm):

@@ -489,66 +489,84 @@ inline SelectPlan select_plan(int64_t groups, int64_t k, int64_t v) {
 }
 
 // ---- reorder -------------------------------------------------------------------------------------------------------------------
-// An item is gp groups x kin beams x cb columns (units of 1 << shift bytes) of one array, at most 64 * kReg units: a wave takes the
-// whole item into registers before it stores any of it, and columns of a row do not depend on each other, so the rows of a group
-// may be permuted in place.
-constexpr int kReorderReg = 8, kReorderMax = 24;
+// An item is gp groups x kout beams x cb columns (units of 1 << shift bytes) of one array, at most 64 * kReorderReg units: a wave takes
+// the whole item into registers before it stores any of it, and columns of a row do not depend on each other, so the rows of a
+// group may be permuted in place.  Rows go in units of 16 bytes at whatever address they start, and what is left of them (below 16
+// bytes) as an array of its own.  Bound by memory: 65 536 envs of 320 bytes in four arrays (42 MB) 11.1 us, 32 rows of 1 MiB (67 MB) 10.5 us;
+// half the loads in flight per wave: 11.9 and 13.0 us.
+constexpr int kReorderReg = 8, kReorderMax = 48;
 struct ReorderArray {
   const uint8_t* src;
   uint8_t* dst;
   int64_t src_stride, dst_stride;  // bytes
   int64_t units;                   // of a row
-  uint32_t first;                  // first item
+  int64_t last;                    // where the last of them starts: it may overlap the one before (an item then holds whole rows)
   uint32_t blocks;                 // column blocks
   int cb, gp, shift;
   uint32_t mul_cb, mul_out;        // t / cb = t * mul_cb >> 21, likewise / beams out (t < 512)
 };
 struct ReorderArgs {
   ReorderArray a[kReorderMax];
+  uint32_t first[kReorderMax];  // first item; 2^32 - 1 behind the last array
   const int32_t* parents;
   int64_t groups;
   uint32_t items;
   int n, kin, kout, in_place;
 };
+static_assert(sizeof(ReorderArgs) <= 4096, "kernel arguments");
+
+template <class U> struct __attribute__((packed, aligned(1))) AnyPlace { U v; };
 
 template <class U> __device__ __forceinline__ void reorder_item(const ReorderArray& a, const ReorderArgs& p, uint32_t item, int lane) {
   const int64_t g0 = (int64_t)(item / a.blocks) * a.gp, c0 = (int64_t)(item % a.blocks) * a.cb;
+  int parent[kReorderReg];
+  int64_t to[kReorderReg];
   U v[kReorderReg];
-  U* to[kReorderReg];
 #pragma unroll
   for (int i = 0; i < kReorderReg; ++i) {
     const uint32_t t = (uint32_t)(i * 64 + lane);
     const uint32_t rg = (t * a.mul_cb) >> 21, c = t - rg * a.cb;        // row of the item, column
     const uint32_t dg = (rg * a.mul_out) >> 21, r = rg - dg * p.kout;   // group of the item, beam
-    const int64_t g = g0 + dg, col = c0 + c;
-    to[i] = nullptr;
-    if ((int)dg < a.gp && g < p.groups && col < a.units) {
-      const int from = p.parents[g * p.kout + r];
-      if (from >= 0 && from < p.kin && !(p.in_place && from == (int)r)) {
-        v[i] = *(const U*)(a.src + (g * p.kin + from) * a.src_stride + (col << a.shift));
-        to[i] = (U*)(a.dst + (g * p.kout + r) * a.dst_stride + (col << a.shift));
-      }
+    const int64_t row = g0 * p.kout + rg;
+    parent[i] = -1;
+    to[i] = 0;
+    if ((int)dg < a.gp && g0 + dg < p.groups && c0 + c < a.units) {
+      const int q = p.parents[row];
+      const int64_t at = (c0 + c) << a.shift;
+      to[i] = row * a.dst_stride + (at < a.last ? at : a.last);
+      parent[i] = p.in_place && q == (int)r ? -1 : q;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kReorderReg; ++i) {
+    const uint32_t t = (uint32_t)(i * 64 + lane);
+    const uint32_t rg = (t * a.mul_cb) >> 21, c = t - rg * a.cb, dg = (rg * a.mul_out) >> 21;
+    if ((uint32_t)parent[i] < (uint32_t)p.kin) {  // (negative ones are large)
+      const int64_t at = (c0 + c) << a.shift;
+      v[i] = ((const AnyPlace<U>*)(a.src + ((g0 + dg) * p.kin + parent[i]) * a.src_stride + (at < a.last ? at : a.last)))->v;
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every load of the wave is back before its first store
 #pragma unroll
   for (int i = 0; i < kReorderReg; ++i)
-    if (to[i]) *to[i] = v[i];
+    if ((uint32_t)parent[i] < (uint32_t)p.kin) ((AnyPlace<U>*)(a.dst + to[i]))->v = v[i];
 }
 
 __global__ __launch_bounds__(256) void reorder_kernel(const ReorderArgs p) {
   const uint32_t item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (item >= p.items) return;
-  int k = 0;
-  while (k + 1 < p.n && item >= p.a[k + 1].first) ++k;
+  int k = -1;
+#pragma unroll
+  for (int i = 0; i < kReorderMax; ++i) k += item >= p.first[i];
   const ReorderArray& a = p.a[k];
   const int lane = threadIdx.x & 63;
+  const uint32_t it = item - p.first[k];
   switch (a.shift) {
-    case 4: reorder_item<v4i>(a, p, item - a.first, lane); break;
-    case 3: reorder_item<uint64_t>(a, p, item - a.first, lane); break;
-    case 2: reorder_item<uint32_t>(a, p, item - a.first, lane); break;
-    case 1: reorder_item<uint16_t>(a, p, item - a.first, lane); break;
-    default: reorder_item<uint8_t>(a, p, item - a.first, lane); break;
+    case 4: reorder_item<v4i>(a, p, it, lane); break;
+    case 3: reorder_item<uint64_t>(a, p, it, lane); break;
+    case 2: reorder_item<uint32_t>(a, p, it, lane); break;
+    case 1: reorder_item<uint16_t>(a, p, it, lane); break;
+    default: reorder_item<uint8_t>(a, p, it, lane); break;
   }
 }
 

@@ -149,6 +149,8 @@ template <class OT, bool U8, int KS> __global__ __launch_bounds__(256) void line
   {
     const int64_t c = n0 + lane < a.n ? n0 + lane : a.n - 1;
     column[wave][lane] = {a.ws[c], a.bias ? a.bias[c] : 0.0f};
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
 #pragma unroll
   for (int s = 0; s < KS; ++s)

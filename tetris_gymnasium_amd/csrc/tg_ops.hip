@@ -285,7 +285,10 @@ int tg_beam_reorder(int device, void* stream, int n, const void* const* src, voi
   if (n == 0 || groups == 0) return TG_OK;
   if (!src || !dst || !row_bytes || !src_stride || !dst_stride || !parents) return fail(TG_EINVAL, "tg_beam_reorder: null pointer");
   if ((uintptr_t)parents % 4) return fail(TG_EINVAL, "tg_beam_reorder: parents not aligned");
-  ReorderArgs p{};
+  static_assert(2 * TG_OPS_MAX_STATES <= kReorderMax, "a row's whole units and its rest");
+  ReorderArgs p;
+  p.n = 0;
+  p.items = 0;
   const int64_t rin = groups * beams_in, rout = groups * beams_out;
   bool in_place = dst[0] == src[0];
   for (int i = 0; i < n; ++i) {
@@ -294,7 +297,7 @@ int tg_beam_reorder(int device, void* stream, int n, const void* const* src, voi
       return fail(TG_EINVAL, "tg_beam_reorder: array %d: rows of %lld bytes at strides %lld / %lld", i, (long long)rb, (long long)ss, (long long)ds);
     if (rb == 0) continue;
     if (!src[i] || !dst[i]) return fail(TG_EINVAL, "tg_beam_reorder: array %d is null", i);
-    const int64_t ns = (rin - 1) * ss + rb, nd = (rout - 1) * ds + rb;
+    const int64_t nd = (rout - 1) * ds + rb;
     if (overlap(dst[i], nd, parents, 4 * rout)) return fail(TG_EINVAL, "tg_beam_reorder: array %d overlaps the parents", i);
     if ((dst[i] == src[i]) != in_place) return fail(TG_EINVAL, "tg_beam_reorder: some arrays in place and some not");
     if (in_place && (ss != ds || beams_in != beams_out)) return fail(TG_EINVAL, "tg_beam_reorder: array %d: in place needs equal strides and beams", i);
@@ -304,29 +307,36 @@ int tg_beam_reorder(int device, void* stream, int n, const void* const* src, voi
           (j != i && overlap(dst[i], nd, dst[j], (rout - 1) * dst_stride[j] + row_bytes[j])))
         return fail(TG_EINVAL, "tg_beam_reorder: arrays %d and %d overlap", i, j);
     }
-    (void)ns;
-    ReorderArray& a = p.a[p.n];
-    a.src = (const uint8_t*)src[i];
-    a.dst = (uint8_t*)dst[i];
-    a.src_stride = ss;
-    a.dst_stride = ds;
-    const uint64_t bits = (uint64_t)(uintptr_t)src[i] | (uintptr_t)dst[i] | (uint64_t)rb | (uint64_t)ss | (uint64_t)ds | 16;
-    a.shift = __builtin_ctzll(bits);
-    a.units = rb >> a.shift;
     const int64_t most = 64 * kReorderReg / beams_out;  // columns of an item of one group
-    a.cb = (int)(a.units < most ? a.units : most);
-    a.gp = (int)(64 * kReorderReg / (beams_out * a.cb));
-    if (a.cb < a.units) a.gp = 1;
-    a.mul_cb = ((1u << 21) + a.cb - 1) / a.cb;
-    a.mul_out = ((1u << 21) + (uint32_t)beams_out - 1) / (uint32_t)beams_out;
-    const int64_t blocks = (a.units + a.cb - 1) / a.cb, items = blocks * ((groups + a.gp - 1) / a.gp);
-    if (blocks > kMaxGrid || items + p.items > kMaxGrid) return fail(TG_EINVAL, "tg_beam_reorder: too much in one call (array %d)", i);
-    a.blocks = (uint32_t)blocks;
-    a.first = p.items;
-    p.items += (uint32_t)items;
-    ++p.n;
+    // Units of 16 bytes; what is left of a row goes as one more unit that overlaps the last where an item holds whole rows (nobody else
+    // reads those bytes then), else as an array of its own in the largest units that divide it.
+    const bool over = rb >= 16 && rb % 16 && (rb + 15) / 16 <= most;
+    const int64_t whole = over ? rb : rb >= 16 ? rb & ~(int64_t)15 : 0;
+    for (const int64_t part : {whole, rb - whole}) {
+      if (part == 0) continue;
+      const int64_t at = part == whole ? 0 : whole;
+      ReorderArray& a = p.a[p.n];
+      a.src = (const uint8_t*)src[i] + at;
+      a.dst = (uint8_t*)dst[i] + at;
+      a.src_stride = ss;
+      a.dst_stride = ds;
+      a.shift = over ? 4 : __builtin_ctzll((uint64_t)part | 16);
+      a.units = (part + (1 << a.shift) - 1) >> a.shift;
+      a.last = part - (1 << a.shift);
+      a.cb = (int)(a.units < most ? a.units : most);
+      a.gp = a.cb < a.units ? 1 : (int)(64 * kReorderReg / (beams_out * a.cb));
+      a.mul_cb = ((1u << 21) + a.cb - 1) / a.cb;
+      a.mul_out = ((1u << 21) + (uint32_t)beams_out - 1) / (uint32_t)beams_out;
+      const int64_t blocks = (a.units + a.cb - 1) / a.cb, sets = (groups + a.gp - 1) / a.gp;
+      if (blocks > kMaxGrid || sets > (kMaxGrid - p.items) / blocks) return fail(TG_EINVAL, "tg_beam_reorder: too much in one call (array %d)", i);
+      a.blocks = (uint32_t)blocks;
+      p.first[p.n] = p.items;
+      p.items += (uint32_t)(blocks * sets);
+      ++p.n;
+    }
   }
   if (p.n == 0) return TG_OK;
+  for (int i = p.n; i < kReorderMax; ++i) p.first[i] = 0xFFFFFFFFu;
   p.parents = parents;
   p.groups = groups;
   p.kin = (int)beams_in;
