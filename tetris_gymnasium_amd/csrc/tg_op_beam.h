@@ -546,7 +546,7 @@ template <class U> __device__ __forceinline__ void reorder_item(const ReorderArr
       v[i] = ((const AnyPlace<U>*)(a.src + ((g0 + dg) * p.kin + parent[i]) * a.src_stride + (at < a.last ? at : a.last)))->v;
     }
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every load of the wave is back before its first store
+  if (p.in_place) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every load of the wave is back before its first store
 #pragma unroll
   for (int i = 0; i < kReorderReg; ++i)
     if ((uint32_t)parent[i] < (uint32_t)p.kin) ((AnyPlace<U>*)(a.dst + to[i]))->v = v[i];
