@@ -86,7 +86,8 @@ int tg_beam_advance(int device, void* stream, int64_t groups, int64_t beams, con
 /* ... and behind the transition: gain += reward, or -inf where the game has ended (n environments). */
 int tg_beam_collect(int device, void* stream, int64_t n, const tg_step_out* out, float* gain);
 
-/* The handle's stream (a hipStream_t), for calls above that shall run in order with the handle's own. */
+/* The handle's stream (a hipStream_t), for calls above that shall run in order with the handle's own.  (tg_config.streams > 1 spreads
+ * transitions over further streams, which this call and every other one on the handle join: ask again behind a transition.) */
 int tg_stream(tg_handle* h, void** stream);
 
 #ifdef __cplusplus

@@ -2,6 +2,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <tuple>
 
 #include "../../include/tetris_gym_hip.h"
 #include "../../include/tetris_gym_ops.h"
@@ -43,9 +44,18 @@ struct DeviceScope {
     return fail(TG_EHIP, name ": device %d: %s (there is no CPU fallback)", device, hipGetErrorString(scope.err)); \
   }
 
-int launched(const char* name) {
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? TG_OK : fail(TG_EHIP, "%s: launch failed: %s", name, hipGetErrorString(e));
+// A launch with its own answer: hipGetLastError would also report what another library left behind on this thread.
+template <class... P, class... A> hipError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t stream, const A&... args) {
+  std::tuple<P...> held{static_cast<P>(args)...};
+  return std::apply([&](P&... p) {
+    void* at[] = {(void*)&p...};
+    return hipLaunchKernel((const void*)kernel, grid, block, at, lds, stream);
+  }, held);
+}
+int launched(const char* name, hipError_t e) {
+  if (e == hipSuccess) return TG_OK;
+  (void)hipGetLastError();
+  return fail(TG_EHIP, "%s: launch failed: %s", name, hipGetErrorString(e));
 }
 
 int type_size(int t) { return t <= kI8 ? 1 : t == kF32 ? 4 : 2; }
@@ -59,7 +69,7 @@ bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
 constexpr int64_t kMost = (int64_t)1 << 40;  // sizes and strides beyond a card's memory: products of two stay in 64 bits below
 constexpr int64_t kMaxGrid = 0x7FFFFFFF;
 
-template <class F> int by_float(int t, F f) {
+template <class F> hipError_t by_float(int t, F f) {
   if (t == kF32) return f(float{});
   if (t == kF16) return f(_Float16{});
   return f(bf16_t{});
@@ -67,7 +77,7 @@ template <class F> int by_float(int t, F f) {
 
 constexpr int kUnits = 256;  // compute units
 
-template <class OT, bool U8, int KS> void linear_rows(const LinearArgs& a, hipStream_t st) {
+template <class OT, bool U8, int KS> hipError_t linear_rows(const LinearArgs& a, hipStream_t st) {
   const int64_t cols = (a.n + 63) / 64;
   const int shift = cols >= 4 ? 2 : cols == 2 ? 1 : 0, below = 4 >> shift;
   const int64_t gy = (cols + (1 << shift) - 1) >> shift, tiles = (a.rows + 15) / 16;
@@ -75,18 +85,17 @@ template <class OT, bool U8, int KS> void linear_rows(const LinearArgs& a, hipSt
   int64_t gx = (kUnits * (KS == 1 ? 3 : 2) + gy - 1) / gy;
   if (gx > (tiles + below - 1) / below) gx = (tiles + below - 1) / below;
   const int64_t inside = a.x_stride ? ((a.rows - 1) * a.x_stride + a.k - 64 * KS) / (16 * a.x_stride) : 0;
-  hipLaunchKernelGGL((linear_rows_kernel<OT, U8, KS>), dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, st, a, shift, inside);
+  return launch(linear_rows_kernel<OT, U8, KS>, dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, st, a, shift, inside);
 }
 
-template <class OT, bool U8, int T, int U> void linear_few(const LinearArgs& a, hipStream_t st) {
+template <class OT, bool U8, int T, int U> hipError_t linear_few(const LinearArgs& a, hipStream_t st) {
   int waves = (int)((a.k + 255) / 256);
   waves = waves < 1 ? 1 : waves > 8 ? 8 : waves;
   const int kw = (int)((a.k + waves * 64 - 1) / (waves * 64)) * 64;
-  hipLaunchKernelGGL((linear_few_kernel<OT, U8, T, U>), dim3((unsigned)((a.n + 16 * T - 1) / (16 * T)), (unsigned)((a.rows + 16 * U - 1) / (16 * U))),
-                     dim3(64 * waves), 0, st, a, kw);
+  return launch(linear_few_kernel<OT, U8, T, U>, dim3((unsigned)((a.n + 16 * T - 1) / (16 * T)), (unsigned)((a.rows + 16 * U - 1) / (16 * U))), dim3(64 * waves), 0, st, a, kw);
 }
 
-template <class OT, bool U8, int BM, int BN, int WM, int WN, bool AL> void linear_tile(const LinearArgs& a, hipStream_t st) {
+template <class OT, bool U8, int BM, int BN, int WM, int WN, bool AL> hipError_t linear_tile(const LinearArgs& a, hipStream_t st) {
   const int64_t mt = (a.rows + BM - 1) / BM, nt = (a.n + BN - 1) / BN;
   const int64_t most = kMaxGrid / nt;  // row tiles of one launch
   for (int64_t i = 0; i < mt; i += most) {
@@ -96,12 +105,14 @@ template <class OT, bool U8, int BM, int BN, int WM, int WN, bool AL> void linea
     b.out = (OT*)a.out + i * BM * a.out_stride;
     b.rows = a.rows - i * BM < most * BM ? a.rows - i * BM : most * BM;
     const int m = (int)((b.rows + BM - 1) / BM);
-    hipLaunchKernelGGL((linear_tile_kernel<OT, U8, BM, BN, WM, WN, AL>), dim3((unsigned)(m * nt)), dim3(WM * WN * 64), 2 * (BM + BN) * 128, st, b, m, (int)nt);
+    const hipError_t e = launch(linear_tile_kernel<OT, U8, BM, BN, WM, WN, AL>, dim3((unsigned)(m * nt)), dim3(WM * WN * 64), 2 * (BM + BN) * 128, st, b, m, (int)nt);
+    if (e != hipSuccess) return e;
   }
+  return hipSuccess;
 }
 
 // Times in us, back to back, bf16 out; rows x k x n.
-template <class OT, bool U8> void linear_launch(const LinearArgs& a, hipStream_t st) {
+template <class OT, bool U8> hipError_t linear_launch(const LinearArgs& a, hipStream_t st) {
   const auto tiles = [&](int64_t bm, int64_t bn) { return ((a.rows + bm - 1) / bm) * ((a.n + bn - 1) / bn); };
   // Few rows: the waves of a workgroup share K.  The widest variant that still gives every compute unit a workgroup: 64 x 4 096 x 8 192:
   // 15.3 (2, 4) against 17.7 (2, 2) and 30.7 (1, 1), but 64 x 1 024 x 1 024: 6.7, 4.8, 3.4.  Above 64 rows only where tiles would leave
@@ -157,19 +168,16 @@ int tg_linear_i8(int device, void* stream, const void* x, int x_type, int64_t ro
     return fail(TG_EINVAL, "tg_linear_i8: the output overlaps an input");
   ON_DEVICE("tg_linear_i8", device);
   LinearArgs a{(const uint8_t*)x, w, w_scale, x_scale, bias, out, rows, k, n, x_stride, w_stride, out_stride, relu != 0};
-  by_float(out_type, [&](auto o) {
+  return launched("tg_linear_i8", by_float(out_type, [&](auto o) {
     using OT = decltype(o);
-    if (x_type == kU8) linear_launch<OT, true>(a, (hipStream_t)stream);
-    else linear_launch<OT, false>(a, (hipStream_t)stream);
-    return 0;
-  });
-  return launched("tg_linear_i8");
+    return x_type == kU8 ? linear_launch<OT, true>(a, (hipStream_t)stream) : linear_launch<OT, false>(a, (hipStream_t)stream);
+  }));
 }
 
 int tg_quantize_i8(int device, void* stream, const void* x, int x_type, int64_t rows, int64_t k, int64_t x_stride, int8_t* q, int64_t q_stride,
                    float* scale) {
   if (!is_float(x_type)) return fail(TG_EINVAL, "tg_quantize_i8: x must be f32, f16 or bf16, got type %d", x_type);
-  if (rows < 0 || k < 0 || rows > ((int64_t)1 << 34) || k > (1 << 30)) return fail(TG_EINVAL, "tg_quantize_i8: bad sizes (rows %lld, k %lld)", (long long)rows, (long long)k);
+  if (rows < 0 || k < 0 || rows > kMaxGrid || k > (1 << 30)) return fail(TG_EINVAL, "tg_quantize_i8: bad sizes (rows %lld, k %lld)", (long long)rows, (long long)k);
   if (rows == 0) return TG_OK;
   if (rows > 1 && (x_stride < 0 || x_stride > (1 << 30) || q_stride < k || q_stride > (1 << 30)))
     return fail(TG_EINVAL, "tg_quantize_i8: row strides (x %lld, q %lld) out of range", (long long)x_stride, (long long)q_stride);
@@ -183,33 +191,24 @@ int tg_quantize_i8(int device, void* stream, const void* x, int x_type, int64_t 
       return fail(TG_EINVAL, "tg_quantize_i8: the outputs overlap each other or the input");
   }
   ON_DEVICE("tg_quantize_i8", device);
-  by_float(x_type, [&](auto e) {
+  return launched("tg_quantize_i8", by_float(x_type, [&](auto e) {
     using T = decltype(e);
     const int64_t vec = kQVec<T>;
-    const auto grid = [&](int rpb) { return dim3((unsigned)((rows + rpb - 1) / rpb)); };
-    const auto run = [&](auto kernel, int rpb) { hipLaunchKernelGGL(kernel, grid(rpb), dim3(256), 0, (hipStream_t)stream, (const T*)x, rows, k, x_stride, q, q_stride, scale); };
     // rows in as few registers as they need: four or sixteen lanes a row, then a wave, then a workgroup
-    if (k <= 4 * vec) run(quantize_kernel<T, 4, 1>, 64);
-    else if (k <= 8 * vec) run(quantize_kernel<T, 4, 2>, 64);
-    else if (k <= 16 * vec) run(quantize_kernel<T, 16, 1>, 16);
-    else if (k <= 32 * vec) run(quantize_kernel<T, 16, 2>, 16);
-    else if (k <= 64 * vec) run(quantize_kernel<T, 16, 4>, 16);
-    else if (k <= 128 * vec) run(quantize_kernel<T, 64, 2>, 4);
-    else if (k <= 256 * vec) run(quantize_kernel<T, 64, 4>, 4);
-    else {
-      for (int64_t r = 0; r < rows; r += kMaxGrid) {
-        const int64_t c = rows - r < kMaxGrid ? rows - r : kMaxGrid;
-        const auto part = [&](auto kernel) {
-          hipLaunchKernelGGL(kernel, dim3((unsigned)c), dim3(256), 0, (hipStream_t)stream, (const T*)x + r * x_stride, c, k, x_stride, q + r * q_stride, q_stride, scale + r);
-        };
-        if (k <= 512 * vec) part(quantize_kernel<T, 256, 2>);
-        else if (k <= 1024 * vec) part(quantize_kernel<T, 256, 4>);
-        else part(quantize_kernel<T, 256, 8>);
-      }
-    }
-    return 0;
-  });
-  return launched("tg_quantize_i8");
+    const auto run = [&](auto kernel, int rpb) {
+      return launch(kernel, dim3((unsigned)((rows + rpb - 1) / rpb)), dim3(256), 0, (hipStream_t)stream, (const T*)x, rows, k, x_stride, q, q_stride, scale);
+    };
+    if (k <= 4 * vec) return run(quantize_kernel<T, 4, 1>, 64);
+    if (k <= 8 * vec) return run(quantize_kernel<T, 4, 2>, 64);
+    if (k <= 16 * vec) return run(quantize_kernel<T, 16, 1>, 16);
+    if (k <= 32 * vec) return run(quantize_kernel<T, 16, 2>, 16);
+    if (k <= 64 * vec) return run(quantize_kernel<T, 16, 4>, 16);
+    if (k <= 128 * vec) return run(quantize_kernel<T, 64, 2>, 4);
+    if (k <= 256 * vec) return run(quantize_kernel<T, 64, 4>, 4);
+    if (k <= 512 * vec) return run(quantize_kernel<T, 256, 2>, 1);
+    if (k <= 1024 * vec) return run(quantize_kernel<T, 256, 4>, 1);
+    return run(quantize_kernel<T, 256, 8>, 1);
+  }));
 }
 
 int64_t tg_beam_select_workspace(int64_t groups, int64_t beams_in, int64_t vocab, int64_t beams_out) {
@@ -252,27 +251,23 @@ int tg_beam_select(int device, void* stream, const void* logits, int type, int64
   }
   ON_DEVICE("tg_beam_select", device);
   const SelectArgs a{logits, scores, mask, finished, out_scores, parents, tokens, lg, lk, mg, mk, groups, (int)beams_in, (int)vocab, (int)beams_out, pad, normalize != 0};
-  by_float(type, [&](auto e) {
+  return launched("tg_beam_select", by_float(type, [&](auto e) {
     using T = decltype(e);
     const hipStream_t st = (hipStream_t)stream;
     if (p.small) {
       const dim3 grid((unsigned)((groups + 3) / 4));
-      if (p.per_lane <= 2) hipLaunchKernelGGL((select_small_kernel<T, 2>), grid, dim3(256), 0, st, a, p.shift);
-      else if (p.per_lane <= 5) hipLaunchKernelGGL((select_small_kernel<T, 5>), grid, dim3(256), 0, st, a, p.shift);
-      else if (p.per_lane <= 8) hipLaunchKernelGGL((select_small_kernel<T, 8>), grid, dim3(256), 0, st, a, p.shift);
-      else hipLaunchKernelGGL((select_small_kernel<T, 16>), grid, dim3(256), 0, st, a, p.shift);
-    } else {
-      const dim3 grid((unsigned)(groups * beams_in * p.chunks));
-      const size_t lds = (size_t)select_list((int)beams_out, p.e) * 8;  // (at most 64 KiB)
-      uint8_t* ws = (uint8_t*)workspace;
-      if (p.e == 8) hipLaunchKernelGGL((select_chunk_kernel<T, 8>), grid, dim3(256), lds, st, a, p.chunks, ws);
-      else if (p.e == 16) hipLaunchKernelGGL((select_chunk_kernel<T, 16>), grid, dim3(256), lds, st, a, p.chunks, ws);
-      else hipLaunchKernelGGL((select_chunk_kernel<T, 32>), grid, dim3(256), lds, st, a, p.chunks, ws);
-      hipLaunchKernelGGL(select_merge_kernel, dim3((unsigned)groups), dim3(256), 0, st, a, p.chunks, (const uint8_t*)ws);
+      if (p.per_lane <= 2) return launch(select_small_kernel<T, 2>, grid, dim3(256), 0, st, a, p.shift);
+      if (p.per_lane <= 5) return launch(select_small_kernel<T, 5>, grid, dim3(256), 0, st, a, p.shift);
+      if (p.per_lane <= 8) return launch(select_small_kernel<T, 8>, grid, dim3(256), 0, st, a, p.shift);
+      return launch(select_small_kernel<T, 16>, grid, dim3(256), 0, st, a, p.shift);
     }
-    return 0;
-  });
-  return launched("tg_beam_select");
+    const dim3 grid((unsigned)(groups * beams_in * p.chunks));
+    const size_t lds = (size_t)select_list((int)beams_out, p.e) * 8;  // (at most 64 KiB)
+    uint8_t* ws = (uint8_t*)workspace;
+    const auto chunks = [&](auto kernel) { return launch(kernel, grid, dim3(256), lds, st, a, p.chunks, ws); };
+    const hipError_t err = p.e == 8 ? chunks(select_chunk_kernel<T, 8>) : p.e == 16 ? chunks(select_chunk_kernel<T, 16>) : chunks(select_chunk_kernel<T, 32>);
+    return err != hipSuccess ? err : launch(select_merge_kernel, dim3((unsigned)groups), dim3(256), 0, st, a, p.chunks, (const uint8_t*)ws);
+  }));
 }
 
 int tg_beam_reorder(int device, void* stream, int n, const void* const* src, void* const* dst, const int64_t* row_bytes,
@@ -343,8 +338,7 @@ int tg_beam_reorder(int device, void* stream, int n, const void* const* src, voi
   p.kout = (int)beams_out;
   p.in_place = in_place;
   ON_DEVICE("tg_beam_reorder", device);
-  hipLaunchKernelGGL(reorder_kernel, dim3((p.items + 3) / 4), dim3(256), 0, (hipStream_t)stream, p);
-  return launched("tg_beam_reorder");
+  return launched("tg_beam_reorder", launch(reorder_kernel, dim3((p.items + 3) / 4), dim3(256), 0, (hipStream_t)stream, p));
 }
 
 int tg_beam_advance(int device, void* stream, int64_t groups, int64_t beams, const int32_t* parents, const int32_t* tokens,
@@ -356,9 +350,7 @@ int tg_beam_advance(int device, void* stream, int64_t groups, int64_t beams, con
   if (!parents || !tokens || !gain_in || !gain_out || !actions) return fail(TG_EINVAL, "tg_beam_advance: null pointer");
   if (overlap(gain_out, 4 * n, gain_in, 4 * n)) return fail(TG_EINVAL, "tg_beam_advance: gain_out overlaps gain_in");
   ON_DEVICE("tg_beam_advance", device);
-  hipLaunchKernelGGL(advance_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, parents, tokens, gain_in, gain_out,
-                     actions, n, (int)beams);
-  return launched("tg_beam_advance");
+  return launched("tg_beam_advance", launch(advance_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, parents, tokens, gain_in, gain_out, actions, n, (int)beams));
 }
 
 int tg_beam_collect(int device, void* stream, int64_t n, const tg_step_out* out, float* gain) {
@@ -366,8 +358,7 @@ int tg_beam_collect(int device, void* stream, int64_t n, const tg_step_out* out,
   if (n == 0) return TG_OK;
   if (!out || !gain) return fail(TG_EINVAL, "tg_beam_collect: null pointer");
   ON_DEVICE("tg_beam_collect", device);
-  hipLaunchKernelGGL(collect_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, out, gain, n);
-  return launched("tg_beam_collect");
+  return launched("tg_beam_collect", launch(collect_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, out, gain, n));
 }
 
 }  // extern "C"
