@@ -56,7 +56,9 @@ int tg_quantize_i8(int device, void* stream, const void* x, int x_type, int64_t 
  * beams_in - 1), tokens i32 (0 .. vocab - 1); equal ones by beam, then by entry; within one beam entries rank by their logit.  Where
  * there are fewer: score -inf, parent -1, token -1.  logits: f32 / f16 / bf16 [groups][beams_in][vocab] (strides lg, lk; lk = 0 or
  * lg = 0 broadcasts), mask likewise (mg, mk), scores / finished [groups][beams_in] and the outputs [groups][beams_out] contiguous.
- * c is held in 64 bits, L to 1e-12.  workspace: tg_beam_select_workspace bytes (0 for small searches), 16-byte
+ * c is held and ranked in 64 bits with L good to 1e-12, and rows of logits that differ by a constant get the same log-probabilities (a single
+ * allowed entry 0): only scores nearer than that to each other may come out in another order than their exact values.
+ * workspace: tg_beam_select_workspace bytes (0 for small searches), 16-byte
  * aligned, not shared by calls that may run at the same time. */
 int64_t tg_beam_select_workspace(int64_t groups, int64_t beams_in, int64_t vocab, int64_t beams_out);
 int tg_beam_select(int device, void* stream, const void* logits, int type, int64_t groups, int64_t beams_in, int64_t vocab, int64_t lg,

@@ -212,7 +212,7 @@ def selected(x, sc, beams, mask=None, done=None, pad=0, norm=True):
             with np.errstate(all="ignore"):
                 if norm and len(e):
                     m = e.max()
-                    e = e - (m + np.log(np.exp(e - m).sum()))
+                    e = (e - m) - np.log(np.exp(e - m).sum())  # (m + log first would lose the logarithm beside a maximum of 3e38)
                 c = float(sc[i, j]) + e
             first = np.argsort(np.where(c > -np.inf, -c, np.inf), kind="stable")[:beams]
             cand += [(-c[o], j, int(at[o])) for o in first if c[o] > -np.inf]
@@ -273,6 +273,30 @@ def test_select_ties_go_to_the_lowest(box, k, v, norm):
     asc = np.tile(np.arange(v, dtype=np.float64) / 64, (2, k, 1))  # the best always comes last / first
     select_case(box, asc, np.zeros((2, k)), 9, norm=norm)
     select_case(box, -asc, np.zeros((2, k)), 9, norm=norm)
+
+
+@pytest.mark.parametrize("k,v", [(26, 2), (8, 40), (4, 1500), (2, 9000)])
+def test_select_forced_moves_keep_their_score(box, k, v):
+    """one allowed entry: log-probability 0 exactly, so equal scores stay equal and go to the lowest beam"""
+    r = np.random.default_rng(v)
+    mask = np.zeros((6, k, v), bool)
+    for i in range(6):
+        mask[i, np.arange(k), r.integers(0, v, k)] = True
+    for dtype in ("float32", "bfloat16"):
+        select_case(box, r.normal(size=(6, k, v)) * 30, -r.integers(0, 3, (6, k)).astype(np.float64), min(k, 9), dtype, mask=mask)
+
+
+@pytest.mark.parametrize("v", [40, 1500, 9000])
+def test_select_rows_that_differ_by_a_constant_tie(box, v):
+    """equal log-probabilities from different logits: the lowest beam first"""
+    r = np.random.default_rng(v)
+    base = np.round(r.normal(size=v) * 4) / 4
+    x = np.stack([base + c for c in (0.0, 1.0, -7.0, 64.0, 0.25)])[None].astype(np.float32)
+    outs = [box.put(np.zeros((1, 20), t)) for t in (np.float32, np.int32, np.int32)]
+    need = ops.beam_select_workspace(1, 5, v, 20)
+    ops.beam_select(box.put(x), box.put(np.zeros((1, 5), np.float32)), *outs, workspace=box.put(np.zeros(need, np.uint8)) if need else None, stream=box.stream)
+    order = np.lexsort((np.arange(5 * v) % v, np.arange(5 * v) // v, -np.tile(base, 5)))[:20]
+    np.testing.assert_array_equal(box.get(outs[1])[0] * v + box.get(outs[2])[0], order)
 
 
 @pytest.mark.parametrize("k,v", [(3, 40), (4, 700), (2, 9000)])

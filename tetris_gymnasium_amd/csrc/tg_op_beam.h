@@ -38,11 +38,16 @@ __device__ __forceinline__ double exp64(double d) {
   return __longlong_as_double((long long)(u + ((uint64_t)(uint32_t)(uint64_t)__double_as_longlong(z) << 52)));
 }
 
-// ln(s) for positive normal s: the hardware's float32 logarithm y, then one step of Newton's method to the third order in what it lacks
-// (s e^-y = 1 + z, |z| < 2^-16: z - z^2/2 leaves z^3/3 < 2e-15); the error is that of exp64.
+// ln(s) for positive normal s = 2^e h, h in [0.7, 1.4): the hardware's float32 logarithm y of h, then one step of Newton's method to the
+// third order in what it lacks (h e^-y = 1 + z, |z| < 2^-16: z - z^2/2 leaves z^3/3 < 2e-15); the error is that of exp64.  ln(1) is 0
+// exactly: a beam with one allowed entry keeps its score.
 __device__ __forceinline__ double log64(double s) {
   int e;
-  const double h = frexp(s, &e);  // (a sum of up to 2^20 terms, but of any magnitude where it is rescaled)
+  double h = frexp(s, &e);
+  if (h < 0.7) {
+    h += h;
+    --e;
+  }
   const double y = (double)(__builtin_amdgcn_logf((float)h) * 0.693147180559945f);
   const double z = fma(h, exp64(-y), -1.0);
   return fma((double)e, 0x1.62e42fefa39efp-1, y + fma(-0.5 * z, z, z));
@@ -197,7 +202,7 @@ template <class T, int N> __global__ __launch_bounds__(256) void select_small_ke
   float e[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) e[i] = here && !done && ok[i] != 0 && sub + i * L < a.v ? to_f32(raw[i]) : -__builtin_inff();
-  double lse = 0;
+  double md = 0, ls = 0;  // the log-sum as maximum + logarithm: (x - md) - ls is the same for rows that differ by a constant
   if (a.norm) {
     float m = -__builtin_inff();
 #pragma unroll
@@ -210,7 +215,7 @@ template <class T, int N> __global__ __launch_bounds__(256) void select_small_ke
     if (L > 16) m = fm(m, xor_lane<16>(m));
     if (L > 32) m = fm(m, xor_lane<32>(m));
     double s = 0;
-    const double md = m;
+    md = m;
     bool nan = m == __builtin_inff();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -224,12 +229,12 @@ template <class T, int N> __global__ __launch_bounds__(256) void select_small_ke
     if (L > 8) s += xor_lane<8>(s);
     if (L > 16) s += xor_lane<16>(s);
     if (L > 32) s += xor_lane<32>(s);
-    lse = md + log64(s);
+    ls = log64(s);
   }
   Cand k[N];
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    k[i] = {e[i] > -__builtin_inff() ? (double)sc + ((double)e[i] - lse) : -__builtin_inf(), e[i], ((uint32_t)jj << 24) + (uint32_t)(sub + i * L)};
+    k[i] = {e[i] > -__builtin_inff() ? (double)sc + (((double)e[i] - md) - ls) : -__builtin_inf(), e[i], ((uint32_t)jj << 24) + (uint32_t)(sub + i * L)};
   if (here && done && sub == 0) k[0] = {(double)sc, 0.0f, ((uint32_t)j << 24) + (uint32_t)a.pad};
   const int64_t o = g * a.beams;
   const int n = wave_top(k, a.beams, lds[wave], [&](int rank, const Key& c) { put_result(a, o + rank, c); });
@@ -386,7 +391,7 @@ __global__ __launch_bounds__(256) void select_merge_kernel(const SelectArgs a, i
   constexpr int N = 4;
   __shared__ Cand lds[64];
   __shared__ Key top[64];
-  __shared__ double lse[64];
+  __shared__ double row_max[64], row_log[64];
   __shared__ float score[64];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int64_t g = blockIdx.x, pb = select_part_bytes(a.beams);
@@ -414,7 +419,7 @@ __global__ __launch_bounds__(256) void select_merge_kernel(const SelectArgs a, i
     if (lane < a.k) {
       score[lane] = a.scores[g * a.k + lane];
       done = a.finished && a.finished[g * a.k + lane];
-      if (!a.norm) lse[lane] = 0;
+      if (!a.norm) row_max[lane] = row_log[lane] = 0;
     }
   }
   if (a.norm) {
@@ -432,7 +437,10 @@ __global__ __launch_bounds__(256) void select_merge_kernel(const SelectArgs a, i
       const float all = group_reduce<64>(m, [](float p, float q) { return fmaxf(p, q); });
       if (s != 0.0) s *= exp64((double)m - (double)all);
       s = group_reduce<64>(s, [](double p, double q) { return p + q; });
-      if (lane == 0) lse[j] = (double)all + log64(s);
+      if (lane == 0) {
+        row_max[j] = all;
+        row_log[j] = log64(s);
+      }
     }
   }
   __syncthreads();
@@ -445,7 +453,7 @@ __global__ __launch_bounds__(256) void select_merge_kernel(const SelectArgs a, i
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float x = unorder_f32((uint32_t)(u[i] >> 32));
-      k[i] = {u[i] ? (double)score[row[i]] + ((double)x - lse[row[i]]) : -__builtin_inf(), x, (row[i] << 24) | ~(uint32_t)u[i]};
+      k[i] = {u[i] ? (double)score[row[i]] + (((double)x - row_max[row[i]]) - row_log[row[i]]) : -__builtin_inf(), x, (row[i] << 24) | ~(uint32_t)u[i]};
       if (found == a.beams && !better(key_of(k[i]), bottom)) k[i].c = -__builtin_inf();
       any |= k[i].c > -__builtin_inf();
     }
