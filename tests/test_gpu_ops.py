@@ -424,3 +424,14 @@ def test_select_sums_over_wide_ranges(box, v, dtype):
         mask[0, 0, -1] = mask[0, 0, 0] = True
         select_case(box, x, sc, 4, dtype)
         select_case(box, x, sc, 4, dtype, mask=mask)
+
+
+@pytest.mark.parametrize("rows", [4, 300])
+def test_linear_without_columns_reads_no_operand(box, rows):
+    """rows of no columns have strides too (1 for an empty array of PyTorch's) and no memory"""
+    b = box.put(np.array([-1, 0, 2], np.float32))
+    out = box.put(np.full((rows, 3), 7, np.float32))
+    for stride in (1, 64):
+        ops.linear_i8(ops.DeviceView(0, (rows, 0), "uint8", (stride, 1)), ops.DeviceView(0, (3, 0), "int8", (stride, 1)), box.put(np.ones(3, np.float32)),
+                      out, bias=b, stream=box.stream)
+        np.testing.assert_array_equal(box.get(out), np.tile(np.array([-1, 0, 2], np.float32), (rows, 1)))

@@ -162,6 +162,7 @@ int tg_linear_i8(int device, void* stream, const void* x, int x_type, int64_t ro
     return fail(TG_EINVAL, "tg_linear_i8: out / w_scale / x_scale / bias not aligned to their elements");
   if (rows == 1) { x_stride = k; out_stride = n; }
   if (n == 1) w_stride = k;
+  if (k == 0) x_stride = w_stride = 0;  // (no operand: strides of empty rows must not span bytes that are not there)
   const int64_t no = span(rows, n, out_stride, os);
   if ((k && (overlap(out, no, x, span(rows, k, x_stride, 1)) || overlap(out, no, w, span(n, k, w_stride, 1)))) || overlap(out, no, w_scale, 4 * n) ||
       overlap(out, no, x_scale, 4 * rows) || overlap(out, no, bias, 4 * n))
