@@ -58,8 +58,8 @@ int tg_quantize_i8(int device, void* stream, const void* x, int x_type, int64_t 
  * lg = 0 broadcasts), mask likewise (mg, mk), scores / finished [groups][beams_in] and the outputs [groups][beams_out] contiguous.
  * c is held and ranked in 64 bits with L good to 1e-12, and rows of logits that differ by a constant get the same log-probabilities (a single
  * allowed entry 0): only scores nearer than that to each other may come out in another order than their exact values.
- * workspace: tg_beam_select_workspace bytes (0 for small searches), 16-byte
- * aligned, not shared by calls that may run at the same time. */
+ * workspace: tg_beam_select_workspace bytes (0 for small searches, TG_EINVAL beyond the limits above), 16-byte aligned, not shared by
+ * calls that may run at the same time and apart from every other array. */
 int64_t tg_beam_select_workspace(int64_t groups, int64_t beams_in, int64_t vocab, int64_t beams_out);
 int tg_beam_select(int device, void* stream, const void* logits, int type, int64_t groups, int64_t beams_in, int64_t vocab, int64_t lg,
                    int64_t lk, const float* scores, const uint8_t* mask, int64_t mg, int64_t mk, const uint8_t* finished, int pad,

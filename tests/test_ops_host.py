@@ -179,3 +179,20 @@ def test_scorer_refusals():
     f = np.array([[1.0, -2.0, 0.25]], np.float32)
     (q, sc, _), = PlacementScorer.from_float([(f, None)]).layers
     assert q.tolist() == [[64, -127, 16]] and sc[0] == np.float32(2.0) / np.float32(127)  # 63.5 to even, 15.875
+
+
+@pytest.mark.parametrize("sizes", [(1, 65, 100, 8), (1, 100, 100000, 8), (1, 8, 100, 65), (1, 8, (1 << 20) + 1, 8), (1 << 31, 8, 100000, 8), (1 << 62, 1, 1, 1)])
+def test_workspace_of_sizes_beyond_the_limits(sizes):
+    with pytest.raises(ValueError, match="are supported"):
+        ops.beam_select_workspace(*sizes)
+
+
+@pytest.mark.parametrize("name", ["logits", "scores", "mask", "finished"])
+def test_select_refuses_a_workspace_over_an_input(name):
+    g, k, v = 1, 4, 100000
+    a = dict(logits=V((g, k, v), "float32"), scores=V((g, k), "float32", at=1 << 24), mask=V((g, k, v), "uint8", at=2 << 24),
+             finished=V((g, k), "uint8", at=3 << 24))
+    ws = ops.DeviceView(a[name].ptr, (ops.beam_select_workspace(g, k, v, 4),), "uint8")
+    with pytest.raises(ValueError, match="workspace overlaps"):
+        ops.beam_select(a["logits"], a["scores"], V((g, 4), "float32", at=4 << 24), V((g, 4), "int32", at=5 << 24), V((g, 4), "int32", at=6 << 24),
+                        mask=a["mask"], finished=a["finished"], workspace=ws)

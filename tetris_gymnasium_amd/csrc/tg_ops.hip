@@ -214,6 +214,9 @@ int tg_quantize_i8(int device, void* stream, const void* x, int x_type, int64_t 
 
 int64_t tg_beam_select_workspace(int64_t groups, int64_t beams_in, int64_t vocab, int64_t beams_out) {
   if (groups < 0 || beams_in < 0 || vocab < 0 || beams_out < 0) return fail(TG_EINVAL, "tg_beam_select_workspace: negative size");
+  if (groups > kMaxGrid || beams_in > TG_OPS_MAX_BEAMS || beams_out > TG_OPS_MAX_BEAMS || vocab > TG_OPS_MAX_VOCAB)
+    return fail(TG_EINVAL, "tg_beam_select_workspace: %lld groups, %lld beams in, %lld out, %lld entries: up to %lld, %d, %d, %d are supported", (long long)groups,
+                (long long)beams_in, (long long)beams_out, (long long)vocab, (long long)kMaxGrid, TG_OPS_MAX_BEAMS, TG_OPS_MAX_BEAMS, TG_OPS_MAX_VOCAB);
   if (groups == 0 || beams_in == 0 || vocab == 0) return 0;
   const SelectPlan p = select_plan(groups, beams_in, vocab);
   return p.small ? 0 : groups * beams_in * p.chunks * select_part_bytes((int)beams_out);
@@ -249,6 +252,9 @@ int tg_beam_select(int device, void* stream, const void* logits, int type, int64
           overlap(outs[i], no, finished, ni / 4) || overlap(outs[i], no, outs[(i + 1) % 3], no) || (need && overlap(outs[i], no, workspace, need)))
         return fail(TG_EINVAL, "tg_beam_select: the outputs overlap each other or an input");
     }
+    if (need && (overlap(workspace, need, logits, nl) || overlap(workspace, need, scores, ni) || (mask && overlap(workspace, need, mask, nm)) ||
+                 overlap(workspace, need, finished, ni / 4)))
+      return fail(TG_EINVAL, "tg_beam_select: the workspace overlaps an input");
   }
   ON_DEVICE("tg_beam_select", device);
   const SelectArgs a{logits, scores, mask, finished, out_scores, parents, tokens, lg, lk, mg, mk, groups, (int)beams_in, (int)vocab, (int)beams_out, pad, normalize != 0};
