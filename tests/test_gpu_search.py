@@ -221,3 +221,18 @@ def test_a_full_game_is_played_longer_than_at_random():
         over |= e.step(np.maximum(s.plan(2)["best"][:, 0], 0))[1] != 0
     assert not over.any()
     s.close(), e.close()
+
+
+def test_deeper_plans_do_not_pile_up_memory():
+    e = Engine(3, 10, 20, obs_mode=N.OBS_BOARD)
+    e.reset(np.array([1, 2, 3], np.uint64))
+    s = BeamSearch(e, linear_scorer(10, 0), 2)
+    first = [s.plan(d) for d in (1, 2)]
+    held = len(s._bufs)
+    deeper = [s.plan(d) for d in (3, 4, 5)]
+    assert len(s._bufs) == held
+    again = s.plan(2)  # shorter ones in the longer buffers
+    for k in first[1]:
+        np.testing.assert_array_equal(again[k], first[1][k])
+    assert [p["actions"].shape[2] for p in deeper] == [3, 4, 5]
+    s.close(), e.close()

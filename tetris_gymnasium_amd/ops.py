@@ -9,7 +9,9 @@ Arrays are device memory of one GPU: a PyTorch tensor, a `DeviceArray` of an Eng
 `__cuda_array_interface__`, or a `DeviceView` around a raw pointer.  Outputs are the caller's; nothing is allocated, kept or
 waited for.  Calls run on `stream` (an integer hipStream_t, e.g. `torch.cuda.current_stream().cuda_stream`; 0 = the default
 stream) in order with whatever else runs there, and may be captured into a graph.  A `DeviceArray` is exported as to any other
-consumer: its engine's stream is waited for first.  Bad arguments raise ValueError, a failed call EngineError."""
+consumer: its engine's stream is waited for first.  A call runs on its arrays' device, whatever the current one is (an array that is
+known by `__cuda_array_interface__` alone does not tell: that of the others, or 0).  Bad arguments raise ValueError, a failed
+call EngineError."""
 from __future__ import annotations
 
 import ctypes as C

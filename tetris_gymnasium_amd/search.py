@@ -152,6 +152,7 @@ class BeamSearch:
             raise ValueError(f"plan: depth must be at least 1, got {depth}")
         e, G, K, st = self.e, self.G, self.beams, self.stream
         if self._steps is None or self._steps[0].shape[0] < depth:
+            self._bufs = [b for b in self._bufs if self._steps is None or b.ptr not in (self._steps[0].ptr, self._steps[1].ptr)]
             self._steps = (self._view((depth, G, K), "int32"), self._view((depth, G, K), "int32"))
         par, tok = self._steps
         self._load()
