@@ -387,13 +387,13 @@ template <class T, int E> __global__ __launch_bounds__(256) void select_chunk_ke
 // through the candidates in rounds of 256, the first entries of all lists before the second ones, so that later rounds soon hold
 // nothing better than the `beams` already found.  Bound by latency (one small workgroup per group): the first round's candidates are
 // asked for at the start.
-__global__ __launch_bounds__(256) void select_merge_kernel(const SelectArgs a, int chunks, const uint8_t* ws) {
+__global__ __launch_bounds__(1024) void select_merge_kernel(const SelectArgs a, int chunks, const uint8_t* ws) {
   constexpr int N = 4;
   __shared__ Cand lds[64];
   __shared__ Key top[64];
   __shared__ double row_max[64], row_log[64];
   __shared__ float score[64];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, waves = blockDim.x >> 6;
   const int64_t g = blockIdx.x, pb = select_part_bytes(a.beams);
   const uint8_t* base = ws + g * a.k * chunks * pb;
   const uint32_t lists = (uint32_t)(a.k * chunks), total = lists * (uint32_t)a.beams;
@@ -423,7 +423,7 @@ __global__ __launch_bounds__(256) void select_merge_kernel(const SelectArgs a, i
     }
   }
   if (a.norm) {
-    for (int j = wave; j < a.k; j += 4) {
+    for (int j = wave; j < a.k; j += waves) {
       float m = -__builtin_inff();
       double s = 0;
       for (int c = lane; c < chunks; c += 64) {

@@ -273,7 +273,7 @@ int tg_beam_select(int device, void* stream, const void* logits, int type, int64
     uint8_t* ws = (uint8_t*)workspace;
     const auto chunks = [&](auto kernel) { return launch(kernel, grid, dim3(256), lds, st, a, p.chunks, ws); };
     const hipError_t err = p.e == 8 ? chunks(select_chunk_kernel<T, 8>) : p.e == 16 ? chunks(select_chunk_kernel<T, 16>) : chunks(select_chunk_kernel<T, 32>);
-    return err != hipSuccess ? err : launch(select_merge_kernel, dim3((unsigned)groups), dim3(256), 0, st, a, p.chunks, (const uint8_t*)ws);
+    return err != hipSuccess ? err : launch(select_merge_kernel, dim3((unsigned)groups), dim3(64 * (!a.norm ? 1 : a.k < 16 ? a.k : 16)), 0, st, a, p.chunks, (const uint8_t*)ws);
   }));
 }
 
