@@ -16,13 +16,22 @@ from . import ops
 from .engine import DeviceBuffer, Engine, EngineError
 
 
+_F16_MAX, _F16_STEP = 65504.0, 2.0**-24
+
+
 class PlacementScorer:
     """A multi-layer perceptron over feature vectors in 8-bit integers: layers of (weight int8 [out, in], scale float32 [out], bias
     float32 [out] or None), relu between them, one output.  The first layer reads the uint8 features, each later one the rows
-    of the layer before quantised to 8 bits."""
+    of the layer before quantised to 8 bits.  Layers whose values could pass the range of float32 are refused.
+
+    `hidden` names the type each hidden layer's activations are kept in.  The quantiser behind them rounds to 1/254 of the row's largest,
+    so float16's relative 2^-11 is an eighth of that and half the bytes of float32; its range is what decides: float16 where no
+    features can take the layer beyond 65 504 and its last step, 2^-24, is not above what one step of one weight adds for
+    one unit of one feature (rounding to it then loses no more than rounding that weight to 8 bits did), else float32."""
 
     def __init__(self, layers):
-        self.layers = []
+        self.layers, self.hidden = [], []
+        reach, least = 255.0, 1.0  # the most an input of the layer can be, and the least step of one (features: bytes)
         for i, (w, s, b) in enumerate(layers):
             w, s = np.asarray(w), np.ascontiguousarray(s, np.float32)
             b = None if b is None else np.ascontiguousarray(b, np.float32)
@@ -33,6 +42,16 @@ class PlacementScorer:
             if self.layers and self.layers[-1][0].shape[0] != w.shape[1]:
                 raise ValueError(f"layer {i} takes {w.shape[1]} inputs, layer {i - 1} gives {self.layers[-1][0].shape[0]}")
             self.layers.append((np.ascontiguousarray(w), s, b))
+            with np.errstate(all="ignore"):
+                # (a weight of 0 counts as 1: the product of the two scales has to be finite too)
+                most = np.maximum(np.abs(w.astype(np.float64)).sum(1), 1) * np.abs(s.astype(np.float64)) * reach
+                most = float(np.max(most if b is None else most + np.abs(b.astype(np.float64)), initial=0.0))
+                least *= float(np.min(np.abs(s), initial=1.0))
+            if not most <= float(np.finfo(np.float32).max):  # (also a scale or a bias that is not a number)
+                raise ValueError(f"layer {i}: its values are not bounded by the range of float32 (up to {most:.3g})")
+            self.hidden.append("float16" if most <= _F16_MAX and least >= _F16_STEP else "float32")
+            reach = most * (1 + 2.0**-10)  # (rounded to its type, then scale times 127)
+        self.hidden = self.hidden[:-1]
         if not self.layers or self.layers[-1][0].shape[0] != 1:
             raise ValueError("a scorer needs at least one layer, and the last one has one output")
 
@@ -93,7 +112,7 @@ class BeamSearch:
         x = self._x
         for i, (w, s, b) in enumerate(scorer.layers):
             last = i + 1 == len(scorer.layers)
-            y = ops.DeviceView(self.values.ptr, (n * V, 1), "float32", device=self.device) if last else f((n * V, w.shape[0]), "float16")
+            y = ops.DeviceView(self.values.ptr, (n * V, 1), "float32", device=self.device) if last else f((n * V, w.shape[0]), scorer.hidden[i])
             q = None if i == 0 else (f((n * V, w.shape[1]), "int8"), f((n * V,), "float32"))
             self._layers.append((x, q, self._put(w), self._put(s), None if b is None else self._put(b), y, not last))
             x = y
