@@ -35,3 +35,35 @@ def test_pad_counts_only_where_beams_may_be_finished():
     accepted(*a, **kw)
     a, kw = select(finished=V((2, 3), "uint8", at=5 << 30), pad=4)
     accepted(*a, **kw)
+
+
+BIG = 2**64
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ops.linear_i8(V((BIG + 4, 8), "uint8"), V((3, 8), "int8", at=1 << 20), V((3,), "float32", at=2 << 20), V((BIG + 4, 3), "float32", at=3 << 20)),
+    lambda: ops.linear_i8(V((2**40, 2**30, 8), "uint8"), V((3, 8), "int8", at=1 << 20), V((3,), "float32", at=2 << 20), V((2**40, 2**30, 3), "float32", at=3 << 20)),
+    lambda: ops.linear_i8(V((4, 8), "uint8", (BIG + 8, 1)), V((3, 8), "int8", at=1 << 20), V((3,), "float32", at=2 << 20), V((4, 3), "float32", at=3 << 20)),
+    lambda: ops.linear_i8(V((4, 8), "uint8"), V((3, 8), "int8", (BIG + 8, 1), at=1 << 20), V((3,), "float32", at=2 << 20), V((4, 3), "float32", at=3 << 20)),
+    lambda: ops.quantize_i8(V((BIG + 4, 8), "float32"), V((BIG + 4, 8), "int8", at=1 << 20), V((BIG + 4,), "float32", at=2 << 20)),
+    lambda: ops.quantize_i8(V((4, 8), "float32", (BIG + 8, 1)), V((4, 8), "int8", at=1 << 20), V((4,), "float32", at=2 << 20)),
+    lambda: select(g=BIG + 2)[0][0](*select(g=BIG + 2)[0][1:]),
+    lambda: select(v=BIG + 5)[0][0](*select(v=BIG + 5)[0][1:]),
+    lambda: ops.beam_select(V((2, 3, 5), "float32", (BIG + 15, 5, 1)), *select()[0][2:]),
+    lambda: ops.beam_select(*select()[0][1:], mask=V((2, 3, 5), "uint8", (BIG + 15, 5, 1), at=5 << 30)),
+    lambda: ops.beam_select_workspace(BIG + 1, 8, 100000, 8),
+    lambda: ops.beam_select_workspace(1, 8, BIG + 100000, 8),
+    lambda: ops.beam_reorder(V((BIG // 2, 4, 8), "uint8"), V((BIG // 2, 4), "int32", at=1 << 30)),
+    lambda: ops.beam_reorder(V((2, 4, BIG + 8), "uint8"), V((2, 4), "int32", at=1 << 30)),
+    lambda: ops.beam_reorder(V((8, 8), "uint8", (BIG + 8, 1)), V((2, 4), "int32", at=1 << 30)),
+    lambda: ops.beam_reorder(V((8, 2**62), "float32"), V((2, 4), "int32", at=1 << 30)),
+])
+def test_sizes_and_strides_are_not_cut_to_64_bits(call):
+    with pytest.raises(ValueError, match="does not fit"):
+        call()
+
+
+def test_negative_sizes_are_refused():
+    for shape in ((-2, -4, 8), (-1, 8), (4, -8)):
+        with pytest.raises(ValueError, match="negative size"):
+            V(shape, "uint8")

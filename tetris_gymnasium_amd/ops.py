@@ -39,6 +39,8 @@ class DeviceView:
         if dtype not in _SIZES:
             raise ValueError(f"DeviceView: unknown dtype {dtype!r}")
         self.ptr, self.shape, self.dtype, self.device = int(ptr), tuple(int(n) for n in shape), dtype, int(device)
+        if any(n < 0 for n in self.shape):
+            raise ValueError(f"DeviceView: negative size in {self.shape}")
         self.strides = _contiguous(self.shape) if strides is None else tuple(int(s) for s in strides)
         if len(self.strides) != len(self.shape):
             raise ValueError("DeviceView: one stride per axis")
@@ -134,6 +136,13 @@ def _check(lib, rc, what):
         raise ValueError(msg) if rc == N.EINVAL else EngineError(msg)
 
 
+def _int64(what, *ints):
+    """sizes and strides as the C entries take them: ctypes would cut what does not fit"""
+    for i in ints:
+        if not -(2**63) <= i < 2**63:
+            raise ValueError(f"{what}: a size or stride of {i} does not fit 64 bits")
+
+
 def _type(name, what, allowed):
     if name not in allowed:
         raise ValueError(f"{what} must be {' / '.join(allowed)}, got {name}")
@@ -224,6 +233,7 @@ def _linear_plan(xm, wm, sm, om, xsm, bm):
         _type(t, "linear_i8: bias", ("float32",))
         _dense(sh, st, (n,), "linear_i8: bias")
         devs.append(d)
+    _int64("linear_i8", rows, k, xs, n, wst[0], os_)
     return _device(*devs), xtype, rows, k, xs, n, wst[0], otype, os_
 
 
@@ -255,12 +265,14 @@ def _quantize_plan(xm, qm, sm):
     if (qrows, qk) != (rows, k):
         raise ValueError(f"quantize_i8: q must have x's shape {xsh}, got {qsh}")
     _dense(ssh, sst, (rows,) if len(ssh) == 1 else xsh[:-1], "quantize_i8: scale")
+    _int64("quantize_i8", rows, k, xs, qs)
     return _device(d0, d1, d2), xtype, rows, k, xs, qs
 
 
 def beam_select_workspace(groups, beams_in, vocab, beams_out):
     """Bytes of device memory beam_select needs as `workspace` for these sizes (0: none)."""
     lib = _lib()
+    _int64("beam_select_workspace", groups, beams_in, vocab, beams_out)
     n = lib.tg_beam_select_workspace(groups, beams_in, vocab, beams_out)
     if n < 0:
         _check(lib, N.EINVAL, "tg_beam_select_workspace")
@@ -343,6 +355,7 @@ def _select_plan(lm, sm, om, pm, tm, mm, fm, wm):
         _dense(sh, st, sh, "beam_select: workspace")
         nws = sh[0]
         devs.append(d)
+    _int64("beam_select", g, v, *lst, *mst, nws)
     return _device(*devs), ltype, g, k, v, lst[0], lst[1], mst[0], mst[1], b, nws
 
 
@@ -364,6 +377,7 @@ def _state(meta, rows, what):
         cols *= k
     flat = _rows(tuple(sh[:lead]) + (1,), tuple(st[:lead]) + (1,), what)
     stride = flat[2] if flat[0] > 1 else cols
+    _int64(what, cols * size, stride * size)
     return cols * size, stride * size, d
 
 
@@ -406,6 +420,7 @@ def _reorder_plan(pm, metas, outs, beams_in):
         raise ValueError(f"beam_reorder: {k} beams in, {b} out: 1 .. {MAX_BEAMS} are supported")
     if outs is None and k != b:
         raise ValueError(f"beam_reorder: in place takes as many beams out ({b}) as in ({k})")
+    _int64("beam_reorder", g * k, g * b)
     num = C.c_int64 * n
     if g == 0:
         return n, 0, g, k, b, C.c_void_p * n, num(), num(), num()
