@@ -74,6 +74,8 @@ def test_finite_scorers_lose_no_placement_to_the_range_of_their_activations():
     sc = PlacementScorer.from_float([(w, np.full(3, 60000.0, np.float32)), (v, None)])
     e = searched(warm=15)
     s = BeamSearch(e, sc, 8)
-    p = s.plan(3)
-    assert np.isfinite(p["scores"]).all() and (p["best"] >= 0).all()
+    legal, over = e.legal_mask().sum(1), (e.get_state()[1]["flags"] & N.F_GAME_OVER) != 0  # (15 placements at random end some of the games)
+    assert (~over).sum() >= 2
+    p = s.plan(1)
+    assert (np.isfinite(p["scores"]).sum(1) == np.minimum(legal, 8))[~over].all() and (p["best"][:, 0] >= 0)[~over].all()
     s.close(), e.close()

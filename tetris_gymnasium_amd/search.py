@@ -138,9 +138,17 @@ class BeamSearch:
         self._bufs = []
         self.e.close()
 
+    def _open(self):
+        """in front of every use of the views: they point into memory, and run on a stream, that close() has given back"""
+        if not getattr(self.e, "h", None):
+            raise EngineError("this BeamSearch has been closed")
+        if not getattr(self.engine, "h", None):
+            raise EngineError("BeamSearch: the engine it searches has been closed")
+
     # -- one search --------------------------------------------------------------------------------
     def _load(self):
         """every beam of group g := env g of the searched engine; the first beam alive at 0, the others dead"""
+        self._open()
         state = self.engine.get_state_device()
         self.engine.sync()  # (the two engines' streams)
         src = [ops.DeviceView(b.ptr, (self.G, n), t, device=self.device) for b, (n, t) in zip(state, self._src)]
@@ -151,6 +159,7 @@ class BeamSearch:
 
     def value_placements(self):
         """The scorer's values of all placements of all beams' current states: float32 [G, beams, 4W] device memory."""
+        self._open()
         st = self.stream
         self.e._chk(self.e.lib.tg_features(self.e.h), "tg_features")
         for x, q, w, s, b, y, relu in self._layers:
@@ -170,6 +179,7 @@ class BeamSearch:
         depth = int(depth)
         if depth < 1:
             raise ValueError(f"plan: depth must be at least 1, got {depth}")
+        self._open()
         e, G, K, st = self.e, self.G, self.beams, self.stream
         if self._steps is None or self._steps[0].shape[0] < depth:
             self._bufs = [b for b in self._bufs if self._steps is None or b.ptr not in (self._steps[0].ptr, self._steps[1].ptr)]
