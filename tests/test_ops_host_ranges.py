@@ -67,3 +67,20 @@ def test_negative_sizes_are_refused():
     for shape in ((-2, -4, 8), (-1, 8), (4, -8)):
         with pytest.raises(ValueError, match="negative size"):
             V(shape, "uint8")
+
+
+class Foreign:
+    """an array of another library's"""
+
+    def __init__(self, shape, typestr, strides=None, at=0, readonly=False):
+        self.__cuda_array_interface__ = {"shape": shape, "typestr": typestr, "strides": strides, "data": (A + at, readonly), "version": 3}
+
+
+def test_foreign_strides_are_whole_elements():
+    q, s = V((4, 8), "int8", at=1 << 20), V((4,), "float32", at=2 << 20)
+    with pytest.raises(ValueError, match="whole elements"):  # (a field of packed records of 34 bytes)
+        ops.quantize_i8(Foreign((4, 8), "<f4", (34, 4)), q, s)
+    with pytest.raises(ValueError, match="whole elements"):
+        ops.quantize_i8(Foreign((4, 8), "<f4", (32, 6)), q, s)
+    accepted(ops.quantize_i8, Foreign((4, 8), "<f4", (36, 4)), q, s)
+    accepted(ops.quantize_i8, Foreign((4, 8), "<f4"), q, s)

@@ -84,6 +84,8 @@ def _get(a):
         raise ValueError(f"unsupported element type {cai['typestr']}")
     shape, item = tuple(cai["shape"]), _SIZES[name]
     st = cai.get("strides")
+    if st is not None and any(s % item for s in st):
+        raise ValueError(f"strides {tuple(st)} of a {name} array are not whole elements")
     st = _contiguous(shape) if st is None else tuple(s // item for s in st)
     return cai["data"][0], (shape, st, name, None)
 
