@@ -84,3 +84,32 @@ def test_foreign_strides_are_whole_elements():
         ops.quantize_i8(Foreign((4, 8), "<f4", (32, 6)), q, s)
     accepted(ops.quantize_i8, Foreign((4, 8), "<f4", (36, 4)), q, s)
     accepted(ops.quantize_i8, Foreign((4, 8), "<f4"), q, s)
+
+
+def test_read_only_outputs_are_refused():
+    f = lambda n, at, shape=(2, 4): Foreign(shape, n, at=at << 20, readonly=True)  # noqa: E731
+    x, w, s = V((2, 8), "uint8"), V((4, 8), "int8", at=1 << 20), V((4,), "float32", at=2 << 20)
+    a = [V((2, 3, 5), "float32"), V((2, 3), "float32", at=1 << 20), V((2, 4), "float32", at=2 << 20), V((2, 4), "int32", at=3 << 20), V((2, 4), "int32", at=4 << 20)]
+    p = V((2, 3), "int32", at=5 << 20)
+    calls = [lambda: ops.linear_i8(x, w, s, f("<f4", 3)), lambda: ops.quantize_i8(V((2, 4), "float32"), f("|i1", 1), V((2,), "float32", at=2 << 20)),
+             lambda: ops.quantize_i8(V((2, 4), "float32"), V((2, 4), "int8", at=1 << 20), f("<f4", 2, (2,))),
+             lambda: ops.beam_select(*a[:2], f("<f4", 2), *a[3:]), lambda: ops.beam_select(*a[:3], f("<i4", 3), a[4]),
+             lambda: ops.beam_select(*a[:4], f("<i4", 4)), lambda: ops.beam_select(*a, workspace=f("|u1", 5, (64,))),
+             lambda: ops.beam_reorder(f("|u1", 1, (6, 8)), p), lambda: ops.beam_reorder(V((6, 8), "uint8"), p, out=f("|u1", 1, (6, 8)))]
+    for call in calls:
+        with pytest.raises(ValueError, match="read-only"):
+            call()
+    accepted(ops.linear_i8, Foreign((2, 8), "|u1", readonly=True), w, s, V((2, 4), "float32", at=3 << 20))  # (an input may be)
+    accepted(ops.beam_reorder, Foreign((6, 8), "|u1", readonly=True), p, out=V((6, 8), "uint8", at=1 << 20))
+
+
+def test_read_only_device_arrays_are_refused_as_outputs():
+    class E:
+        h, cfg = object(), type("C", (), {"device": 0})
+
+        def sync(self):
+            raise AssertionError("refused before anything waits")
+
+    r = ops.DeviceArray(E(), A, (6, 8), "uint8", readonly=True)
+    with pytest.raises(ValueError, match="read-only"):
+        ops.beam_reorder(r, V((2, 3), "int32", at=5 << 20))

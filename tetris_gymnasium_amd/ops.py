@@ -61,12 +61,14 @@ def _contiguous(shape):
 _plans: dict = {}
 
 
-def _get(a):
+def _get(a, write=False):
     if hasattr(a, "data_ptr"):  # a torch tensor (torch is not imported here)
         return a.data_ptr(), (a.shape, a.stride(), a.dtype, a.get_device())
     if isinstance(a, DeviceView):
         return a.ptr, a._meta
     if isinstance(a, DeviceArray):
+        if write and a._readonly:
+            raise ValueError("an output is a read-only DeviceArray")
         a._ready()
         name, item = a.dtype.name, a.dtype.itemsize
         if a.strides is None:
@@ -79,6 +81,8 @@ def _get(a):
     cai = getattr(a, "__cuda_array_interface__", None)
     if cai is None:
         raise ValueError(f"a device array is needed (torch tensor, DeviceArray, DeviceView or __cuda_array_interface__), got {type(a).__name__}")
+    if write and cai["data"][1]:
+        raise ValueError("an output's __cuda_array_interface__ says that it is read-only")
     name = _STR.get(cai["typestr"])
     if name is None:
         raise ValueError(f"unsupported element type {cai['typestr']}")
@@ -196,7 +200,7 @@ def linear_i8(x, weight, weight_scale, out, *, x_scale=None, bias=None, relu=Fal
     xp, xm = _get(x)
     wp, wm = _get(weight)
     sp, sm = _get(weight_scale)
-    op, om = _get(out)
+    op, om = _get(out, True)
     xsp, xsm = (None, None) if x_scale is None else _get(x_scale)
     bp, bm = (None, None) if bias is None else _get(bias)
     dev, xtype, rows, k, xs, n, wst, otype, os_ = _plan(("linear", xm, wm, sm, om, xsm, bm), _linear_plan, xm, wm, sm, om, xsm, bm)
@@ -245,8 +249,8 @@ def quantize_i8(x, q, scale, *, stream=0):
     x float32 / float16 / bfloat16 [..., K], q int8 [..., K], scale float32 [rows].  q * scale is x to half a step.  A row with a
     NaN or an infinity gets scale NaN and q 0: what is computed from it is NaN, not a plausible number.  Returns (q, scale)."""
     xp, xm = _get(x)
-    qp, qm = _get(q)
-    sp, sm = _get(scale)
+    qp, qm = _get(q, True)
+    sp, sm = _get(scale, True)
     dev, xtype, rows, k, xs, qs = _plan(("quantize", xm, qm, sm), _quantize_plan, xm, qm, sm)
     lib = _lib()
     rc = lib.tg_quantize_i8(dev, stream, xp, xtype, rows, k, xs, qp, qs, sp)
@@ -294,12 +298,12 @@ def beam_select(logits, scores, out_scores, parents, tokens, *, mask=None, finis
     Returns (out_scores, parents, tokens)."""
     lp, lm = _get(logits)
     sp, sm = _get(scores)
-    op, om = _get(out_scores)
-    pp, pm = _get(parents)
-    tp, tm = _get(tokens)
+    op, om = _get(out_scores, True)
+    pp, pm = _get(parents, True)
+    tp, tm = _get(tokens, True)
     mp, mm = (None, None) if mask is None else _get(mask)
     fp, fm = (None, None) if finished is None else _get(finished)
-    wp, wm = (None, None) if workspace is None else _get(workspace)
+    wp, wm = (None, None) if workspace is None else _get(workspace, True)
     dev, ltype, g, k, v, lg, lk, mg, mk, b, nws = _plan(("select", lm, sm, om, pm, tm, mm, fm, wm), _select_plan, lm, sm, om, pm, tm, mm, fm, wm)
     pad = int(pad)
     if finished is None:
@@ -392,8 +396,8 @@ def beam_reorder(states, parents, *, out=None, beams_in=None, stream=0):
     A parent outside 0 .. K - 1 (the -1 of a missing beam) leaves its row as it was.  Returns out (or states)."""
     src = states if isinstance(states, (list, tuple)) else (states,)
     pp, pm = _get(parents)
-    sv = [_get(a) for a in src]
-    dv = sv if out is None else [_get(a) for a in (out if isinstance(out, (list, tuple)) else (out,))]
+    sv = [_get(a, out is None) for a in src]
+    dv = sv if out is None else [_get(a, True) for a in (out if isinstance(out, (list, tuple)) else (out,))]
     metas = tuple([m for _, m in sv])
     outs = None if out is None else tuple([m for _, m in dv])
     n, dev, g, k, b, ptrs, rows, ss, ds = _plan(("reorder", pm, metas, outs, beams_in), _reorder_plan, pm, metas, outs, beams_in)
