@@ -113,3 +113,15 @@ def test_read_only_device_arrays_are_refused_as_outputs():
     r = ops.DeviceArray(E(), A, (6, 8), "uint8", readonly=True)
     with pytest.raises(ValueError, match="read-only"):
         ops.beam_reorder(r, V((2, 3), "int32", at=5 << 20))
+
+
+def test_empty_states_do_not_decide_what_is_in_place():
+    """empty tensors of PyTorch's stand at address 0, sources and outputs alike"""
+    p = V((2, 3), "int32", at=9 << 20)
+    empty, x, y = ops.DeviceView(0, (6, 0), "uint8"), V((6, 8), "uint8"), V((6, 8), "uint8", at=1 << 20)
+    accepted(ops.beam_reorder, [empty, x], p, out=[empty, y])
+    accepted(ops.beam_reorder, [x, empty], p, out=[y, empty])
+    accepted(ops.beam_reorder, [ops.DeviceView(A + 7, (6, 0), "uint8"), x], p, out=[ops.DeviceView(A + 9, (6, 0), "uint8"), x])
+    ops.beam_reorder([empty, empty], p, out=[empty, empty])  # nothing to move
+    with pytest.raises(ValueError, match="some arrays in place"):
+        ops.beam_reorder([empty, x, y], p, out=[empty, x, V((6, 8), "uint8", at=2 << 20)])

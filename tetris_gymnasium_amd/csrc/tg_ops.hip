@@ -292,13 +292,15 @@ int tg_beam_reorder(int device, void* stream, int n, const void* const* src, voi
   p.n = 0;
   p.items = 0;
   const int64_t rin = groups * beams_in, rout = groups * beams_out;
-  bool in_place = dst[0] == src[0];
+  bool in_place = false, first = true;  // (by the first array that has bytes: an empty one may stand at any address)
   for (int i = 0; i < n; ++i) {
     const int64_t rb = row_bytes[i], ss = src_stride[i], ds = dst_stride[i];
     if (rb < 0 || rb > kMost || ss < rb || ds < rb || ss > kMost / 64 || ds > kMost / 64)
       return fail(TG_EINVAL, "tg_beam_reorder: array %d: rows of %lld bytes at strides %lld / %lld", i, (long long)rb, (long long)ss, (long long)ds);
     if (rb == 0) continue;
     if (!src[i] || !dst[i]) return fail(TG_EINVAL, "tg_beam_reorder: array %d is null", i);
+    if (first) in_place = dst[i] == src[i];
+    first = false;
     const int64_t nd = (rout - 1) * ds + rb;
     if (overlap(dst[i], nd, parents, 4 * rout)) return fail(TG_EINVAL, "tg_beam_reorder: array %d overlaps the parents", i);
     if ((dst[i] == src[i]) != in_place) return fail(TG_EINVAL, "tg_beam_reorder: some arrays in place and some not");
