@@ -125,3 +125,23 @@ def test_empty_states_do_not_decide_what_is_in_place():
     ops.beam_reorder([empty, empty], p, out=[empty, empty])  # nothing to move
     with pytest.raises(ValueError, match="some arrays in place"):
         ops.beam_reorder([empty, x, y], p, out=[empty, x, V((6, 8), "uint8", at=2 << 20)])
+
+
+@pytest.mark.parametrize("call", [
+    # 2^31 groups at a stride of 2^40 - 1: the product leaves 64 bits (and comes back as a small or a negative number)
+    lambda: ops.beam_select(V((2**31 - 1, 3, 5), "float32", (2**40, 5, 1)), V((2**31 - 1, 3), "float32", at=1 << 42), V((2**31 - 1, 4), "float32", at=2 << 42),
+                            V((2**31 - 1, 4), "int32", at=3 << 42), V((2**31 - 1, 4), "int32", at=4 << 42)),
+    lambda: ops.beam_select(V((2**24 + 1, 3, 5), "float32", (2**40, 5, 1)), V((2**24 + 1, 3), "float32", at=1 << 42), V((2**24 + 1, 4), "float32", at=2 << 42),
+                            V((2**24 + 1, 4), "int32", at=3 << 42), V((2**24 + 1, 4), "int32", at=4 << 42)),
+    lambda: ops.beam_select(V((2**24 + 1, 3, 5), "float32"), V((2**24 + 1, 3), "float32", at=1 << 42), V((2**24 + 1, 4), "float32", at=2 << 42),
+                            V((2**24 + 1, 4), "int32", at=3 << 42), V((2**24 + 1, 4), "int32", at=4 << 42),
+                            mask=V((2**24 + 1, 3, 5), "uint8", (2**40, 5, 1), at=5 << 42)),
+    lambda: ops.beam_reorder(V((2**30 * 64, 8), "uint8", (2**34, 1)), V((2**30, 64), "int32", at=1 << 44)),
+    lambda: ops.beam_reorder(V((2**30, 8), "uint8"), V((2**24, 64), "int32", at=1 << 44), out=V((2**30, 8), "uint8", (2**34, 1), at=1 << 50)),
+    lambda: ops.quantize_i8(V((2**31 - 1, 8), "float32", (2**30, 1)), V((2**31 - 1, 8), "int8", at=1 << 43), V((2**31 - 1,), "float32", at=1 << 44)),
+    lambda: ops.linear_i8(V((2**34, 8), "uint8", (2**24, 1)), V((3, 8), "int8", at=1 << 45), V((3,), "float32", at=2 << 45), V((2**34, 3), "float32", at=3 << 45)),
+])
+def test_arrays_that_no_memory_holds_are_refused(call):
+    """... before anything is computed from where they end"""
+    with pytest.raises(ValueError, match=r"2\^47 bytes"):
+        call()

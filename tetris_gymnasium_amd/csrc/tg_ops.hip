@@ -61,12 +61,18 @@ int launched(const char* name, hipError_t e) {
 int type_size(int t) { return t <= kI8 ? 1 : t == kF32 ? 4 : 2; }
 bool is_float(int t) { return t == kF32 || t == kF16 || t == kBF16; }
 
-// bytes from the first to behind the last element of [rows][cols] with a row stride (rows, cols > 0)
-int64_t span(int64_t rows, int64_t cols, int64_t stride, int64_t size) { return ((rows - 1) * stride + cols) * size; }
+// Bytes from the first to behind the last element of [rows][cols] with a row stride, or of [groups][rows][cols] with a group stride too
+// (sizes > 0, strides >= 0); -1 where they pass the 2^47 bytes that addresses reach: no memory holds such an array, and sums with it
+// would leave 64 bits.
+constexpr int64_t kAddresses = (int64_t)1 << 47;
+int64_t span(int64_t rows, int64_t cols, int64_t stride, int64_t size, int64_t groups = 1, int64_t group_stride = 0) {
+  const __int128 n = ((__int128)(groups - 1) * group_stride + (__int128)(rows - 1) * stride + cols) * size;
+  return n > kAddresses ? -1 : (int64_t)n;
+}
 bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
   return a && b && (const char*)a < (const char*)b + nb && (const char*)b < (const char*)a + na;
 }
-constexpr int64_t kMost = (int64_t)1 << 40;  // sizes and strides beyond a card's memory: products of two stay in 64 bits below
+constexpr int64_t kMost = (int64_t)1 << 40;  // sizes and strides beyond a card's memory (what products of them reach: span)
 constexpr int64_t kMaxGrid = 0x7FFFFFFF;
 
 template <class F> hipError_t by_float(int t, F f) {
@@ -163,8 +169,9 @@ int tg_linear_i8(int device, void* stream, const void* x, int x_type, int64_t ro
   if (rows == 1) { x_stride = k; out_stride = n; }
   if (n == 1) w_stride = k;
   if (k == 0) x_stride = w_stride = 0;  // (no operand: strides of empty rows must not span bytes that are not there)
-  const int64_t no = span(rows, n, out_stride, os);
-  if ((k && (overlap(out, no, x, span(rows, k, x_stride, 1)) || overlap(out, no, w, span(n, k, w_stride, 1)))) || overlap(out, no, w_scale, 4 * n) ||
+  const int64_t no = span(rows, n, out_stride, os), nx = k ? span(rows, k, x_stride, 1) : 0, nw = k ? span(n, k, w_stride, 1) : 0;
+  if (no < 0 || nx < 0 || nw < 0) return fail(TG_EINVAL, "tg_linear_i8: an array of more than 2^47 bytes");
+  if ((k && (overlap(out, no, x, nx) || overlap(out, no, w, nw))) || overlap(out, no, w_scale, 4 * n) ||
       overlap(out, no, x_scale, 4 * rows) || overlap(out, no, bias, 4 * n))
     return fail(TG_EINVAL, "tg_linear_i8: the output overlaps an input");
   ON_DEVICE("tg_linear_i8", device);
@@ -188,6 +195,7 @@ int tg_quantize_i8(int device, void* stream, const void* x, int x_type, int64_t 
   if (rows == 1) { x_stride = k; q_stride = k; }
   if (k) {
     const int64_t nx = span(rows, k, x_stride, size), nq = span(rows, k, q_stride, 1);
+    if (nx < 0 || nq < 0) return fail(TG_EINVAL, "tg_quantize_i8: an array of more than 2^47 bytes");
     if (overlap(q, nq, x, nx) || overlap(scale, 4 * rows, x, nx) || overlap(scale, 4 * rows, q, nq))
       return fail(TG_EINVAL, "tg_quantize_i8: the outputs overlap each other or the input");
   }
@@ -245,7 +253,8 @@ int tg_beam_select(int device, void* stream, const void* logits, int type, int64
     return fail(TG_EINVAL, "tg_beam_select: a 16-byte aligned workspace of %lld bytes is needed, got %lld", (long long)need, (long long)workspace_bytes);
   {
     const int64_t no = 4 * groups * beams_out, ni = 4 * groups * beams_in;
-    const int64_t nl = ((groups - 1) * lg + (beams_in - 1) * lk + vocab) * type_size(type), nm = (groups - 1) * mg + (beams_in - 1) * mk + vocab;
+    const int64_t nl = span(beams_in, vocab, lk, type_size(type), groups, lg), nm = mask ? span(beams_in, vocab, mk, 1, groups, mg) : 0;
+    if (nl < 0 || nm < 0) return fail(TG_EINVAL, "tg_beam_select: an array of more than 2^47 bytes");
     const void* outs[3] = {out_scores, parents, tokens};
     for (int i = 0; i < 3; ++i) {
       if (overlap(outs[i], no, logits, nl) || overlap(outs[i], no, scores, ni) || (mask && overlap(outs[i], no, mask, nm)) ||
@@ -292,23 +301,27 @@ int tg_beam_reorder(int device, void* stream, int n, const void* const* src, voi
   p.n = 0;
   p.items = 0;
   const int64_t rin = groups * beams_in, rout = groups * beams_out;
-  bool in_place = false, first = true;  // (by the first array that has bytes: an empty one may stand at any address)
   for (int i = 0; i < n; ++i) {
     const int64_t rb = row_bytes[i], ss = src_stride[i], ds = dst_stride[i];
     if (rb < 0 || rb > kMost || ss < rb || ds < rb || ss > kMost / 64 || ds > kMost / 64)
       return fail(TG_EINVAL, "tg_beam_reorder: array %d: rows of %lld bytes at strides %lld / %lld", i, (long long)rb, (long long)ss, (long long)ds);
+    if (rb && (span(rin, rb, ss, 1) < 0 || span(rout, rb, ds, 1) < 0)) return fail(TG_EINVAL, "tg_beam_reorder: array %d: more than 2^47 bytes", i);
+  }
+  bool in_place = false, first = true;  // (by the first array that has bytes: an empty one may stand at any address)
+  for (int i = 0; i < n; ++i) {
+    const int64_t rb = row_bytes[i], ss = src_stride[i], ds = dst_stride[i];
     if (rb == 0) continue;
     if (!src[i] || !dst[i]) return fail(TG_EINVAL, "tg_beam_reorder: array %d is null", i);
     if (first) in_place = dst[i] == src[i];
     first = false;
-    const int64_t nd = (rout - 1) * ds + rb;
+    const int64_t nd = span(rout, rb, ds, 1);
     if (overlap(dst[i], nd, parents, 4 * rout)) return fail(TG_EINVAL, "tg_beam_reorder: array %d overlaps the parents", i);
     if ((dst[i] == src[i]) != in_place) return fail(TG_EINVAL, "tg_beam_reorder: some arrays in place and some not");
     if (in_place && (ss != ds || beams_in != beams_out)) return fail(TG_EINVAL, "tg_beam_reorder: array %d: in place needs equal strides and beams", i);
     for (int j = 0; j < n; ++j) {
-      if (row_bytes[j] <= 0 || (in_place && j == i)) continue;
-      if (overlap(dst[i], nd, src[j], (rin - 1) * src_stride[j] + row_bytes[j]) ||
-          (j != i && overlap(dst[i], nd, dst[j], (rout - 1) * dst_stride[j] + row_bytes[j])))
+      if (row_bytes[j] == 0 || (in_place && j == i)) continue;
+      if (overlap(dst[i], nd, src[j], span(rin, row_bytes[j], src_stride[j], 1)) ||
+          (j != i && overlap(dst[i], nd, dst[j], span(rout, row_bytes[j], dst_stride[j], 1))))
         return fail(TG_EINVAL, "tg_beam_reorder: arrays %d and %d overlap", i, j);
     }
     const int64_t most = 64 * kReorderReg / beams_out;  // columns of an item of one group
