@@ -145,3 +145,18 @@ def test_arrays_that_no_memory_holds_are_refused(call):
     """... before anything is computed from where they end"""
     with pytest.raises(ValueError, match=r"2\^47 bytes"):
         call()
+
+
+def test_more_environments_than_a_launch_holds():
+    lib = N.load()
+    assert lib.tg_beam_advance(0, None, 2**26, 64, 64, 128, 192, 1 << 40, 256) == N.EINVAL  # (a thread each)
+    assert b"environments are supported" in lib.tg_ops_last_error()
+    assert lib.tg_beam_collect(0, None, 2**31, 64, 128) == N.EINVAL
+
+
+def test_sizes_that_need_several_launches_are_accepted():
+    g = 2**18 + 1  # x 64 beams of 17 entries: more chunks than one launch has blocks
+    need = ops.beam_select_workspace(g, 64, 17, 1)
+    a, kw = select(g=g, k=64, v=17, b=1, workspace=V((need,), "uint8", at=1 << 40))
+    accepted(*a, **kw)
+    accepted(ops.quantize_i8, V((2**31 - 1, 1), "float16"), V((2**31 - 1, 1), "int8", at=1 << 40), V((2**31 - 1,), "float32", at=1 << 41))

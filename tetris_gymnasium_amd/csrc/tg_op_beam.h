@@ -521,6 +521,7 @@ struct ReorderArgs {
   const int32_t* parents;
   int64_t groups;
   uint32_t items;
+  uint32_t base;  // the launch's first item
   int n, kin, kout, in_place;
 };
 static_assert(sizeof(ReorderArgs) <= 4096, "kernel arguments");
@@ -563,7 +564,7 @@ template <class U> __device__ __forceinline__ void reorder_item(const ReorderArr
 }
 
 __global__ __launch_bounds__(256) void reorder_kernel(const ReorderArgs p) {
-  const uint32_t item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t item = p.base + blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (item >= p.items) return;
   int k = -1;
 #pragma unroll

@@ -1,4 +1,5 @@
 // Host side of the operators' C ABI (include/tetris_gym_ops.h): checks, choice of a kernel, launch.
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -73,7 +74,10 @@ bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
   return a && b && (const char*)a < (const char*)b + nb && (const char*)b < (const char*)a + na;
 }
 constexpr int64_t kMost = (int64_t)1 << 40;  // sizes and strides beyond a card's memory (what products of them reach: span)
-constexpr int64_t kMaxGrid = 0x7FFFFFFF;
+constexpr int64_t kMaxGroups = 0x7FFFFFFF;
+// A launch holds fewer than 2^32 threads along x, whatever the blocks are (hipLaunchKernel refuses more): calls that need more are
+// spread over several launches.
+constexpr int64_t max_blocks(int threads) { return (int64_t)0xFFFFFFFF / threads; }
 
 template <class F> hipError_t by_float(int t, F f) {
   if (t == kF32) return f(float{});
@@ -103,7 +107,7 @@ template <class OT, bool U8, int T, int U> hipError_t linear_few(const LinearArg
 
 template <class OT, bool U8, int BM, int BN, int WM, int WN, bool AL> hipError_t linear_tile(const LinearArgs& a, hipStream_t st) {
   const int64_t mt = (a.rows + BM - 1) / BM, nt = (a.n + BN - 1) / BN;
-  const int64_t most = kMaxGrid / nt;  // row tiles of one launch
+  const int64_t most = max_blocks(WM * WN * 64) / nt;  // row tiles of one launch (nt <= 2^16)
   for (int64_t i = 0; i < mt; i += most) {
     LinearArgs b = a;
     b.x = a.x + i * BM * a.x_stride;
@@ -185,7 +189,7 @@ int tg_linear_i8(int device, void* stream, const void* x, int x_type, int64_t ro
 int tg_quantize_i8(int device, void* stream, const void* x, int x_type, int64_t rows, int64_t k, int64_t x_stride, int8_t* q, int64_t q_stride,
                    float* scale) {
   if (!is_float(x_type)) return fail(TG_EINVAL, "tg_quantize_i8: x must be f32, f16 or bf16, got type %d", x_type);
-  if (rows < 0 || k < 0 || rows > kMaxGrid || k > (1 << 30)) return fail(TG_EINVAL, "tg_quantize_i8: bad sizes (rows %lld, k %lld)", (long long)rows, (long long)k);
+  if (rows < 0 || k < 0 || rows > kMaxGroups || k > (1 << 30)) return fail(TG_EINVAL, "tg_quantize_i8: bad sizes (rows %lld, k %lld)", (long long)rows, (long long)k);
   if (rows == 0) return TG_OK;
   if (rows > 1 && (x_stride < 0 || x_stride > (1 << 30) || q_stride < k || q_stride > (1 << 30)))
     return fail(TG_EINVAL, "tg_quantize_i8: row strides (x %lld, q %lld) out of range", (long long)x_stride, (long long)q_stride);
@@ -205,7 +209,14 @@ int tg_quantize_i8(int device, void* stream, const void* x, int x_type, int64_t 
     const int64_t vec = kQVec<T>;
     // rows in as few registers as they need: four or sixteen lanes a row, then a wave, then a workgroup
     const auto run = [&](auto kernel, int rpb) {
-      return launch(kernel, dim3((unsigned)((rows + rpb - 1) / rpb)), dim3(256), 0, (hipStream_t)stream, (const T*)x, rows, k, x_stride, q, q_stride, scale);
+      const int64_t most = max_blocks(256) * rpb;
+      for (int64_t r = 0; r < rows; r += most) {
+        const int64_t m = rows - r < most ? rows - r : most;
+        const hipError_t err = launch(kernel, dim3((unsigned)((m + rpb - 1) / rpb)), dim3(256), 0, (hipStream_t)stream, (const T*)x + r * x_stride, m, k, x_stride,
+                                      q + r * q_stride, q_stride, scale + r);
+        if (err != hipSuccess) return err;
+      }
+      return hipSuccess;
     };
     if (k <= 4 * vec) return run(quantize_kernel<T, 4, 1>, 64);
     if (k <= 8 * vec) return run(quantize_kernel<T, 4, 2>, 64);
@@ -222,9 +233,9 @@ int tg_quantize_i8(int device, void* stream, const void* x, int x_type, int64_t 
 
 int64_t tg_beam_select_workspace(int64_t groups, int64_t beams_in, int64_t vocab, int64_t beams_out) {
   if (groups < 0 || beams_in < 0 || vocab < 0 || beams_out < 0) return fail(TG_EINVAL, "tg_beam_select_workspace: negative size");
-  if (groups > kMaxGrid || beams_in > TG_OPS_MAX_BEAMS || beams_out > TG_OPS_MAX_BEAMS || vocab > TG_OPS_MAX_VOCAB)
+  if (groups > kMaxGroups || beams_in > TG_OPS_MAX_BEAMS || beams_out > TG_OPS_MAX_BEAMS || vocab > TG_OPS_MAX_VOCAB)
     return fail(TG_EINVAL, "tg_beam_select_workspace: %lld groups, %lld beams in, %lld out, %lld entries: up to %lld, %d, %d, %d are supported", (long long)groups,
-                (long long)beams_in, (long long)beams_out, (long long)vocab, (long long)kMaxGrid, TG_OPS_MAX_BEAMS, TG_OPS_MAX_BEAMS, TG_OPS_MAX_VOCAB);
+                (long long)beams_in, (long long)beams_out, (long long)vocab, (long long)kMaxGroups, TG_OPS_MAX_BEAMS, TG_OPS_MAX_BEAMS, TG_OPS_MAX_VOCAB);
   if (groups == 0 || beams_in == 0 || vocab == 0) return 0;
   const SelectPlan p = select_plan(groups, beams_in, vocab);
   return p.small ? 0 : groups * beams_in * p.chunks * select_part_bytes((int)beams_out);
@@ -235,7 +246,7 @@ int tg_beam_select(int device, void* stream, const void* logits, int type, int64
                    int normalize, int64_t beams_out, float* out_scores, int32_t* parents, int32_t* tokens, void* workspace,
                    int64_t workspace_bytes) {
   if (!is_float(type)) return fail(TG_EINVAL, "tg_beam_select: logits must be f32, f16 or bf16, got type %d", type);
-  if (groups < 0 || groups > kMaxGrid) return fail(TG_EINVAL, "tg_beam_select: %lld groups", (long long)groups);
+  if (groups < 0 || groups > kMaxGroups) return fail(TG_EINVAL, "tg_beam_select: %lld groups", (long long)groups);
   if (beams_in < 1 || beams_in > TG_OPS_MAX_BEAMS || beams_out < 1 || beams_out > TG_OPS_MAX_BEAMS)
     return fail(TG_EINVAL, "tg_beam_select: %lld beams in, %lld out: 1 .. %d are supported", (long long)beams_in, (long long)beams_out, TG_OPS_MAX_BEAMS);
   if (vocab < 1 || vocab > TG_OPS_MAX_VOCAB) return fail(TG_EINVAL, "tg_beam_select: %lld entries: 1 .. %d are supported", (long long)vocab, TG_OPS_MAX_VOCAB);
@@ -247,7 +258,6 @@ int tg_beam_select(int device, void* stream, const void* logits, int type, int64
   if ((uintptr_t)logits % type_size(type) || (uintptr_t)scores % 4 || (uintptr_t)out_scores % 4 || (uintptr_t)parents % 4 || (uintptr_t)tokens % 4)
     return fail(TG_EINVAL, "tg_beam_select: an array is not aligned to its elements");
   const SelectPlan p = select_plan(groups, beams_in, vocab);
-  if (!p.small && groups * beams_in * p.chunks > kMaxGrid) return fail(TG_EINVAL, "tg_beam_select: %lld groups x %lld beams x %lld entries: too much in one call", (long long)groups, (long long)beams_in, (long long)vocab);
   const int64_t need = tg_beam_select_workspace(groups, beams_in, vocab, beams_out);
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
     return fail(TG_EINVAL, "tg_beam_select: a 16-byte aligned workspace of %lld bytes is needed, got %lld", (long long)need, (long long)workspace_bytes);
@@ -266,9 +276,15 @@ int tg_beam_select(int device, void* stream, const void* logits, int type, int64
       return fail(TG_EINVAL, "tg_beam_select: the workspace overlaps an input");
   }
   ON_DEVICE("tg_beam_select", device);
-  const SelectArgs a{logits, scores, mask, finished, out_scores, parents, tokens, lg, lk, mg, mk, groups, (int)beams_in, (int)vocab, (int)beams_out, pad, normalize != 0};
-  return launched("tg_beam_select", by_float(type, [&](auto e) {
+  const int merge_threads = 64 * (!normalize ? 1 : beams_in < 16 ? (int)beams_in : 16);
+  int64_t most = max_blocks(256) * 4;  // groups of one launch
+  if (!p.small) most = std::min(max_blocks(256) / (beams_in * p.chunks), max_blocks(merge_threads));
+  // (some groups of it, for one launch of each kernel)
+  const auto run = [&](auto e, int64_t g, int64_t groups) {
     using T = decltype(e);
+    const SelectArgs a{(const T*)logits + g * lg, scores + g * beams_in, mask ? mask + g * mg : nullptr, finished ? finished + g * beams_in : nullptr,
+                       out_scores + g * beams_out, parents + g * beams_out, tokens + g * beams_out, lg, lk, mg, mk, groups, (int)beams_in, (int)vocab,
+                       (int)beams_out, pad, normalize != 0};
     const hipStream_t st = (hipStream_t)stream;
     if (p.small) {
       const dim3 grid((unsigned)((groups + 3) / 4));
@@ -279,10 +295,17 @@ int tg_beam_select(int device, void* stream, const void* logits, int type, int64
     }
     const dim3 grid((unsigned)(groups * beams_in * p.chunks));
     const size_t lds = (size_t)select_list((int)beams_out, p.e) * 8;  // (at most 64 KiB)
-    uint8_t* ws = (uint8_t*)workspace;
+    uint8_t* ws = (uint8_t*)workspace + g * beams_in * p.chunks * select_part_bytes((int)beams_out);
     const auto chunks = [&](auto kernel) { return launch(kernel, grid, dim3(256), lds, st, a, p.chunks, ws); };
     const hipError_t err = p.e == 8 ? chunks(select_chunk_kernel<T, 8>) : p.e == 16 ? chunks(select_chunk_kernel<T, 16>) : chunks(select_chunk_kernel<T, 32>);
-    return err != hipSuccess ? err : launch(select_merge_kernel, dim3((unsigned)groups), dim3(64 * (!a.norm ? 1 : a.k < 16 ? a.k : 16)), 0, st, a, p.chunks, (const uint8_t*)ws);
+    return err != hipSuccess ? err : launch(select_merge_kernel, dim3((unsigned)groups), dim3(merge_threads), 0, st, a, p.chunks, (const uint8_t*)ws);
+  };
+  return launched("tg_beam_select", by_float(type, [&](auto e) {
+    for (int64_t g = 0; g < groups; g += most) {
+      const hipError_t err = run(e, g, groups - g < most ? groups - g : most);
+      if (err != hipSuccess) return err;
+    }
+    return hipSuccess;
   }));
 }
 
@@ -290,7 +313,7 @@ int tg_beam_reorder(int device, void* stream, int n, const void* const* src, voi
                     const int64_t* src_stride, const int64_t* dst_stride, int64_t groups, int64_t beams_in, int64_t beams_out,
                     const int32_t* parents) {
   if (n < 0 || n > TG_OPS_MAX_STATES) return fail(TG_EINVAL, "tg_beam_reorder: %d arrays: up to %d go into one call", n, TG_OPS_MAX_STATES);
-  if (groups < 0 || groups > kMaxGrid) return fail(TG_EINVAL, "tg_beam_reorder: %lld groups", (long long)groups);
+  if (groups < 0 || groups > kMaxGroups) return fail(TG_EINVAL, "tg_beam_reorder: %lld groups", (long long)groups);
   if (beams_in < 1 || beams_in > TG_OPS_MAX_BEAMS || beams_out < 1 || beams_out > TG_OPS_MAX_BEAMS)
     return fail(TG_EINVAL, "tg_beam_reorder: %lld beams in, %lld out: 1 .. %d are supported", (long long)beams_in, (long long)beams_out, TG_OPS_MAX_BEAMS);
   if (n == 0 || groups == 0) return TG_OK;
@@ -345,7 +368,7 @@ int tg_beam_reorder(int device, void* stream, int n, const void* const* src, voi
       a.mul_cb = ((1u << 21) + a.cb - 1) / a.cb;
       a.mul_out = ((1u << 21) + (uint32_t)beams_out - 1) / (uint32_t)beams_out;
       const int64_t blocks = (a.units + a.cb - 1) / a.cb, sets = (groups + a.gp - 1) / a.gp;
-      if (blocks > kMaxGrid || sets > (kMaxGrid - p.items) / blocks) return fail(TG_EINVAL, "tg_beam_reorder: too much in one call (array %d)", i);
+      if (blocks > kMaxGroups || sets > (kMaxGroups - p.items) / blocks) return fail(TG_EINVAL, "tg_beam_reorder: too much in one call (array %d)", i);
       a.blocks = (uint32_t)blocks;
       p.first[p.n] = p.items;
       p.items += (uint32_t)(blocks * sets);
@@ -360,14 +383,19 @@ int tg_beam_reorder(int device, void* stream, int n, const void* const* src, voi
   p.kout = (int)beams_out;
   p.in_place = in_place;
   ON_DEVICE("tg_beam_reorder", device);
-  return launched("tg_beam_reorder", launch(reorder_kernel, dim3((p.items + 3) / 4), dim3(256), 0, (hipStream_t)stream, p));
+  hipError_t err = hipSuccess;
+  const uint32_t most = (uint32_t)(4 * max_blocks(256));  // items of one launch
+  for (p.base = 0; err == hipSuccess && p.base < p.items; p.base += most)
+    err = launch(reorder_kernel, dim3((std::min(p.items - p.base, most) + 3) / 4), dim3(256), 0, (hipStream_t)stream, p);
+  return launched("tg_beam_reorder", err);
 }
 
 int tg_beam_advance(int device, void* stream, int64_t groups, int64_t beams, const int32_t* parents, const int32_t* tokens,
                     const float* gain_in, float* gain_out, int32_t* actions) {
-  if (groups < 0 || groups > kMaxGrid || beams < 1 || beams > TG_OPS_MAX_BEAMS)
+  if (groups < 0 || groups > kMaxGroups || beams < 1 || beams > TG_OPS_MAX_BEAMS)
     return fail(TG_EINVAL, "tg_beam_advance: %lld groups of %lld beams", (long long)groups, (long long)beams);
   const int64_t n = groups * beams;
+  if (n > 256 * max_blocks(256)) return fail(TG_EINVAL, "tg_beam_advance: %lld groups of %lld beams: up to %lld environments are supported", (long long)groups, (long long)beams, (long long)(256 * max_blocks(256)));
   if (n == 0) return TG_OK;
   if (!parents || !tokens || !gain_in || !gain_out || !actions) return fail(TG_EINVAL, "tg_beam_advance: null pointer");
   if (overlap(gain_out, 4 * n, gain_in, 4 * n)) return fail(TG_EINVAL, "tg_beam_advance: gain_out overlaps gain_in");
@@ -376,7 +404,7 @@ int tg_beam_advance(int device, void* stream, int64_t groups, int64_t beams, con
 }
 
 int tg_beam_collect(int device, void* stream, int64_t n, const tg_step_out* out, float* gain) {
-  if (n < 0 || n > kMaxGrid) return fail(TG_EINVAL, "tg_beam_collect: %lld environments", (long long)n);
+  if (n < 0 || n > kMaxGroups) return fail(TG_EINVAL, "tg_beam_collect: %lld environments", (long long)n);
   if (n == 0) return TG_OK;
   if (!out || !gain) return fail(TG_EINVAL, "tg_beam_collect: null pointer");
   ON_DEVICE("tg_beam_collect", device);
