@@ -75,8 +75,8 @@ bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
 }
 constexpr int64_t kMost = (int64_t)1 << 40;  // sizes and strides beyond a card's memory (what products of them reach: span)
 constexpr int64_t kMaxGroups = 0x7FFFFFFF;
-// A launch holds fewer than 2^32 threads along x, whatever the blocks are (hipLaunchKernel refuses more): calls that need more are
-// spread over several launches.
+// A launch holds fewer than 2^32 threads along x, whatever the blocks are (with more, hipLaunchKernel has returned success here and run a
+// part of the blocks): calls that need more are spread over several launches.
 constexpr int64_t max_blocks(int threads) { return (int64_t)0xFFFFFFFF / threads; }
 
 template <class F> hipError_t by_float(int t, F f) {
