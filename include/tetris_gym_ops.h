@@ -5,8 +5,8 @@
  *
  * Every pointer is DEVICE memory of `device` unless it says host.  Calls are asynchronous on `stream` (a hipStream_t; NULL =
  * the default stream), allocate nothing, keep nothing, and can be captured into a graph.  They return 0 or a TG_E* code of
- * tetris_gym_hip.h; the message of the calling thread's last failure is tg_ops_last_error().  The caller's current device is
- * left as it was.  Strides count elements; the innermost axis is contiguous.
+ * tetris_gym_hip.h; the message of the calling thread's last failure is tg_ops_last_error() (of the calls that take a handle it is
+ * tg_last_error(handle) too).  The caller's current device is left as it was.  Strides count elements; the innermost axis is contiguous.
  */
 #ifndef TETRIS_GYM_OPS_H
 #define TETRIS_GYM_OPS_H

@@ -79,3 +79,13 @@ def test_finite_scorers_lose_no_placement_to_the_range_of_their_activations():
     p = s.plan(1)
     assert (np.isfinite(p["scores"]).sum(1) == np.minimum(legal, 8))[~over].all() and (p["best"][:, 0] >= 0)[~over].all()
     s.close(), e.close()
+
+
+def test_refusals_of_reorder_beams_are_the_operators_messages_too():
+    e = Engine(12, 10, 20, obs_mode=N.OBS_BOARD)
+    lib = e.lib
+    for beams, parents, msg in ((5, 64, b"divide the batch"), (4, None, b"null parents"), (4, 64, b"never reset")):  # (refused before the address is used)
+        assert lib.tg_reorder_beams(e.h, parents, beams) == N.EINVAL
+        assert msg in lib.tg_ops_last_error() and msg in lib.tg_last_error(e.h)
+    assert lib.tg_stream(e.h, None) == N.EINVAL and lib.tg_ops_last_error().startswith(b"tg_stream")
+    e.close()

@@ -160,3 +160,11 @@ def test_sizes_that_need_several_launches_are_accepted():
     a, kw = select(g=g, k=64, v=17, b=1, workspace=V((need,), "uint8", at=1 << 40))
     accepted(*a, **kw)
     accepted(ops.quantize_i8, V((2**31 - 1, 1), "float16"), V((2**31 - 1, 1), "int8", at=1 << 40), V((2**31 - 1,), "float32", at=1 << 41))
+
+
+def test_calls_on_a_handle_leave_their_message_too():
+    lib = N.load()
+    for name, call in (("tg_stream", lambda: lib.tg_stream(None, None)), ("tg_reorder_beams", lambda: lib.tg_reorder_beams(None, None, 1))):
+        assert lib.tg_beam_collect(0, None, -1, None, None) == N.EINVAL  # an older message
+        assert call() == N.EINVAL
+        assert lib.tg_ops_last_error().decode().startswith(name)

@@ -2182,8 +2182,27 @@ int tg_features(tg_handle* h) {
 }
 
 #ifndef TG_LEGACY_KERNELS  // (the operators are not part of the test-only legacy library)
-int tg_stream(tg_handle* h, void** stream) {
-  if (!h || !stream) return TG_EINVAL;
+}  // extern "C"
+namespace tg { namespace ops { __attribute__((visibility("hidden"))) void set_error(const char* msg); } }  // tg_ops.hip: tg_ops_last_error's text
+namespace {
+
+// A call of tetris_gym_ops.h on a handle: as the others there it leaves the caller's current device as it was and its message in
+// tg_ops_last_error (besides the handle's own).
+template <class F> int ops_call(tg_handle* h, const char* name, F f) {
+  if (!h) {
+    tg::ops::set_error((std::string(name) + ": null handle").c_str());
+    return TG_EINVAL;
+  }
+  int before = -1;
+  if (hipGetDevice(&before) != hipSuccess) before = -1;
+  const int rc = f();
+  if (rc != TG_OK) tg::ops::set_error(h->err.c_str());
+  if (before >= 0) (void)hipSetDevice(before);
+  return rc;
+}
+
+int stream_of(tg_handle* h, void** stream) {
+  if (!stream) return fail(h, TG_EINVAL, "tg_stream: null pointer");
   HIPCHK(h, hipSetDevice(h->cfg.device));
   { int rcj = join_shards(h); if (rcj != TG_OK) return rcj; }
   *stream = h->stream;
@@ -2193,8 +2212,7 @@ int tg_stream(tg_handle* h, void** stream) {
 // Every array a transition reads or a caller sees is one row per env (the double-buffered ones: one row per env and parity), so the
 // state of the whole handle moves in one launch.  What is derived on demand (legal mask, host pack, features) is not state, and
 // a packed handle's stale uint8 board stays as stale as it was.
-int tg_reorder_beams(tg_handle* h, const int32_t* parents, int beams) {
-  if (!h) return TG_EINVAL;
+int reorder_beams(tg_handle* h, const int32_t* parents, int beams) {
   if (!parents) return fail(h, TG_EINVAL, "tg_reorder_beams: null parents");
   if (beams < 1 || beams > TG_OPS_MAX_BEAMS || h->B % beams)
     return fail(h, TG_EINVAL, "tg_reorder_beams: %d beams: 1 .. %d that divide the batch of %d are supported", beams, TG_OPS_MAX_BEAMS, h->B);
@@ -2235,6 +2253,17 @@ int tg_reorder_beams(tg_handle* h, const int32_t* parents, int beams) {
   }
   const int rc = tg_beam_reorder(h->cfg.device, h->stream, n, at, at, bytes, bytes, bytes, h->B / beams, beams, beams, parents);
   return rc == TG_OK ? TG_OK : fail(h, rc, "tg_reorder_beams: %s", tg_ops_last_error());
+}
+
+}  // namespace
+extern "C" {
+
+int tg_stream(tg_handle* h, void** stream) {
+  return ops_call(h, "tg_stream", [&] { return stream_of(h, stream); });
+}
+
+int tg_reorder_beams(tg_handle* h, const int32_t* parents, int beams) {
+  return ops_call(h, "tg_reorder_beams", [&] { return reorder_beams(h, parents, beams); });
 }
 #endif
 

@@ -150,6 +150,8 @@ template <class OT, bool U8> hipError_t linear_launch(const LinearArgs& a, hipSt
 
 }  // namespace
 
+namespace tg { namespace ops { __attribute__((visibility("hidden"))) void set_error(const char* msg) { snprintf(g_err, sizeof(g_err), "%s", msg); } } }
+
 extern "C" {
 
 const char* tg_ops_last_error(void) { return g_err; }
