@@ -81,20 +81,20 @@ __device__ __forceinline__ float lane_f32(float v, int l) { return __uint_as_flo
 
 // A bound that at least `beams` (or all) of the wave's lane maxima reach: with up to 16 beams the beams-th largest of the 16 maxima of
 // four lanes, else of the 64 lane maxima, by counting for each how many are larger.  m = -inf: the lane has nothing; none then passes
-// a bound above -inf.  For T = float and uint64_t.
-template <class T> __device__ __forceinline__ T wave_bound(T m, int beams, T (*lane)(T, int), T top) {
-  auto hi = [](T a, T b) { return a > b ? a : b; };
+// a bound above -inf.
+__device__ __forceinline__ float wave_bound(float m, int beams) {
+  auto hi = [](float a, float b) { return a > b ? a : b; };
   const bool quads = beams <= 16;
   if (quads) m = group_reduce<4>(m, hi);
   int larger = 0;
   if (quads) {
 #pragma unroll
-    for (int l = 0; l < 64; l += 4) larger += lane(m, l) > m;
+    for (int l = 0; l < 64; l += 4) larger += lane_f32(m, l) > m;
   } else {
-    for (int l = 0; l < 64; ++l) larger += lane(m, l) > m;
+    for (int l = 0; l < 64; ++l) larger += lane_f32(m, l) > m;
   }
   // of the values with fewer than `beams` larger ones the smallest: equal values count once, so this is never above the beams-th
-  return group_reduce<64>(larger < beams ? m : top, [](T a, T b) { return a < b ? a : b; });
+  return group_reduce<64>(larger < beams ? m : __builtin_inff(), [](float a, float b) { return a < b ? a : b; });
 }
 
 // A candidate before it is ranked: its score (-inf or NaN: none), its logit, and its beam and entry (row << 24 | entry).
@@ -114,7 +114,7 @@ template <int N, class F> __device__ __forceinline__ int wave_top(const Cand (&k
     c[i] = k[i].c > -__builtin_inf() ? fmaxf((float)k[i].c, low) : -__builtin_inff();
     m = fmaxf(m, c[i]);
   }
-  const float bound = fmaxf(wave_bound<float>(m, beams, lane_f32, __builtin_inff()), low);
+  const float bound = fmaxf(wave_bound(m, beams), low);
   int n = 0, at[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -244,17 +244,18 @@ template <class T, int N> __global__ __launch_bounds__(256) void select_small_ke
 // Large searches, first step: a workgroup per (beam, chunk of 256 * E entries), the chunk in registers: its maximum, its sum of
 // exponentials against that maximum, and its best `beams` entries by (logit, place).  32 x 8 x 32 768 in bf16 (17 MB): 14.5 us, 7 of them
 // the issue of 944 vector instructions per wave (5 us without the exponentials, 3 without the list); chunks of 4 096: 15.0, 2 048: 18.0.
-// Keys are unique, so `beams` quads of lanes (17 and more: lanes) of a wave reach its bound, with all their E entries at most.
-__device__ __host__ __forceinline__ int select_list(int beams, int e) {
-  const int lanes = 4 * beams * (beams <= 16 ? 4 : 1);
-  return (lanes < 256 ? lanes : 256) * e;
-}
+// What reaches a wave's bound is ranked by counting, so the list is kept short: where many equal logits (a clipped or a constant row), rising
+// ones or many beams bring more than kSelectList entries, every wave first narrows its bound until at most kSelectWave remain.
+// 32 x 8 x 32 768 in bf16, whole calls at 8, 16, 64 beams: random logits 20, 37, 114 us, all equal 44, 53, 363 (ranking the
+// whole chunk instead: 7 930 and 8 250 at 16 and 64).
+constexpr int kSelectList = 256, kSelectWave = kSelectList / 4;
+static_assert(kSelectWave >= TG_OPS_MAX_BEAMS, "a wave lists its best `beams` at least");
 struct SelectPart { double s; float m; int n; };  // then uint64_t[beams]: order(logit) << 32 | ~entry, descending, n of them
 __device__ __host__ __forceinline__ int64_t select_part_bytes(int beams) { return 16 + 8 * (int64_t)beams; }
 
 template <class T, int E> __global__ __launch_bounds__(256) void select_chunk_kernel(const SelectArgs a, int chunks, uint8_t* ws) {
   constexpr int V = 16 / (int)sizeof(T), NV = E / V;
-  extern __shared__ uint64_t list[];  // select_list(beams, E): what reaches its wave's bound
+  __shared__ uint64_t list[kSelectList];
   __shared__ float wm[4];
   __shared__ double wsum[4];
   __shared__ int count;
@@ -340,37 +341,62 @@ template <class T, int E> __global__ __launch_bounds__(256) void select_chunk_ke
     s = group_reduce<64>(s, [](double p, double q) { return p + q; });
     if (lane == 0) wsum[wave] = s;
   }
-  // What reaches the wave's bound is listed.  The bound goes by the logit alone first; only where equal logits bring more than the list
-  // holds, it is drawn again over (logit, place), which are all different.
+  // what reaches the wave's bound is listed, as (logit, place)
   auto entry = [&](int i) { return v0 + (i / V) * 256 * V + i % V; };
   auto key = [&](float f, int v) { return ((uint64_t)order_f32(f) << 32) | (uint32_t)~v; };
-  const int room = select_list(a.beams, E);
-  const float bf = fmaxf(wave_bound<float>(lm, a.beams, lane_f32, __builtin_inff()), -3.402823466e38f);
+  const float bf = fmaxf(wave_bound(lm, a.beams), -3.402823466e38f);
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     const bool in = e[i] >= bf;
     if (__ballot(in)) {
       if (in) {
         const int at = atomicAdd(&count, 1);
-        if (at < room) list[at] = key(e[i], entry(i));
+        if (at < kSelectList) list[at] = key(e[i], entry(i));
       }
     }
   }
   __syncthreads();
-  if (count > room) {
+  if (count > kSelectList) {
     __syncthreads();
     if (t == 0) count = 0;
     __syncthreads();
-    uint64_t best = 0;
+    // The bound rises, by halving what lies between it and the wave's largest, as long as `beams` entries reach it; where it ends among
+    // equal logits with too many of them, those behind a place that is found likewise stay out.
+    auto reach = [&](auto in) {
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < E; ++i) n += (int)__popcll(__ballot(in(i)));
+      return n;
+    };
+    float f = bf;
+    int last = 256 * E, n = reach([&](int i) { return e[i] >= f; });
+    uint32_t lo = order_f32(bf), hi = order_f32(group_reduce<64>(lm, [](float p, float q) { return fmaxf(p, q); }));
+    while (n > kSelectWave && lo < hi) {
+      const uint32_t mid = lo + (hi - lo + 1) / 2;
+      const float g = unorder_f32(mid);
+      const int more = reach([&](int i) { return e[i] >= g; });
+      if (more >= a.beams) {
+        lo = mid;
+        f = g;
+        n = more;
+      } else {
+        hi = mid - 1;
+      }
+    }
+    if (n > kSelectWave) {  // (fewer than `beams` are above f: it cannot rise)
+      const int want = a.beams - reach([&](int i) { return e[i] > f; });
+      int from = chunk * (256 * E), to = from + 256 * E - 1;  // the place of the want-th of those at f
+      while (from < to) {
+        const int mid = from + (to - from) / 2;
+        const int in_lane = mid - v0;  // (against a constant for each entry)
+        if (reach([&](int i) { return e[i] == f && (i / V) * 256 * V + i % V <= in_lane; }) >= want) to = mid;
+        else from = mid + 1;
+      }
+      last = to - v0;
+    }
 #pragma unroll
     for (int i = 0; i < E; ++i)
-      if (e[i] > -__builtin_inff()) best = max_u64(best, key(e[i], entry(i)));
-    const uint64_t bound = max_u64(wave_bound<uint64_t>(best, a.beams, lane_u64, ~(uint64_t)0), 1);
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const uint64_t k = e[i] > -__builtin_inff() ? key(e[i], entry(i)) : 0;
-      if (k >= bound) list[atomicAdd(&count, 1)] = k;
-    }
+      if (e[i] > f || (e[i] == f && (i / V) * 256 * V + i % V <= last)) list[atomicAdd(&count, 1)] = key(e[i], entry(i));
   }
   __syncthreads();
   const int n = count, keep = n < a.beams ? n : a.beams;

@@ -296,9 +296,8 @@ int tg_beam_select(int device, void* stream, const void* logits, int type, int64
       return launch(select_small_kernel<T, 16>, grid, dim3(256), 0, st, a, p.shift);
     }
     const dim3 grid((unsigned)(groups * beams_in * p.chunks));
-    const size_t lds = (size_t)select_list((int)beams_out, p.e) * 8;  // (at most 64 KiB)
     uint8_t* ws = (uint8_t*)workspace + g * beams_in * p.chunks * select_part_bytes((int)beams_out);
-    const auto chunks = [&](auto kernel) { return launch(kernel, grid, dim3(256), lds, st, a, p.chunks, ws); };
+    const auto chunks = [&](auto kernel) { return launch(kernel, grid, dim3(256), 0, st, a, p.chunks, ws); };
     const hipError_t err = p.e == 8 ? chunks(select_chunk_kernel<T, 8>) : p.e == 16 ? chunks(select_chunk_kernel<T, 16>) : chunks(select_chunk_kernel<T, 32>);
     return err != hipSuccess ? err : launch(select_merge_kernel, dim3((unsigned)groups), dim3(merge_threads), 0, st, a, p.chunks, (const uint8_t*)ws);
   };
