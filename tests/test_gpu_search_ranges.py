@@ -2,7 +2,8 @@
 import numpy as np
 import pytest
 
-from tetris_gymnasium_amd import BeamSearch, Engine, PlacementScorer, _native as N
+import test_gpu_search
+from tetris_gymnasium_amd import BeamSearch, Engine, PlacementScorer, _native as N, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -88,4 +89,26 @@ def test_refusals_of_reorder_beams_are_the_operators_messages_too():
         assert lib.tg_reorder_beams(e.h, parents, beams) == N.EINVAL
         assert msg in lib.tg_ops_last_error() and msg in lib.tg_last_error(e.h)
     assert lib.tg_stream(e.h, None) == N.EINVAL and lib.tg_ops_last_error().startswith(b"tg_stream")
+    e.close()
+
+
+@pytest.mark.parametrize("w,h,G,K,depth,warm", [(10, 20, 4, 17, 4, 3), (10, 20, 5, 32, 4, 0), (10, 20, 3, 64, 3, 5), (20, 40, 3, 8, 4, 2), (20, 40, 2, 16, 5, 0),
+                                                (32, 24, 2, 5, 3, 0), (4, 12, 3, 33, 3, 0)])
+def test_plans_of_many_beams_and_wide_boards(w, h, G, K, depth, warm, monkeypatch):
+    """searches whose selection takes chunks and a workspace (17 and more beams of 40 placements, 16 of 80), and both sides of that"""
+    e = Engine(G, w, h, obs_mode=N.OBS_BOARD, grouped=True)
+    s = BeamSearch(e, test_gpu_search.linear_scorer(w, K), K)
+    assert (s._ws is not None) == (ops.beam_select_workspace(G, K, 4 * w, K) > 0)
+    s.close(), e.close()
+    test_gpu_search.test_plan_is_the_search_done_on_the_host(w, h, G, K, depth, warm, 0, monkeypatch)
+
+
+def test_the_search_outlives_games_at_random():
+    """the scorer of test_a_full_game_is_played_longer_than_at_random against uniform legal placements on the same games"""
+    e = Engine(8, 10, 20, obs_mode=N.OBS_BOARD, grouped=True)
+    e.reset(np.arange(1, 9, dtype=np.uint64))
+    over = np.zeros(8, bool)
+    for t in range(40):
+        over |= e.step(e.sample_legal_actions(seed=5, counter=t))[1] != 0
+    assert over.any()  # (the search ends none of the eight in 40 placements)
     e.close()
