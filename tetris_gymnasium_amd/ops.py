@@ -305,11 +305,12 @@ def beam_select(logits, scores, out_scores, parents, tokens, *, mask=None, finis
     fp, fm = (None, None) if finished is None else _get(finished)
     wp, wm = (None, None) if workspace is None else _get(workspace, True)
     dev, ltype, g, k, v, lg, lk, mg, mk, b, nws = _plan(("select", lm, sm, om, pm, tm, mm, fm, wm), _select_plan, lm, sm, om, pm, tm, mm, fm, wm)
-    pad = int(pad)
     if finished is None:
         pad = 0
-    elif not 0 <= pad < v:  # (here, not only behind ctypes, which would cut it to 32 bits)
-        raise ValueError(f"beam_select: pad {pad} outside the {v} entries")
+    else:
+        pad = int(pad)
+        if not 0 <= pad < v:  # (here, not only behind ctypes, which would cut it to 32 bits)
+            raise ValueError(f"beam_select: pad {pad} outside the {v} entries")
     lib = _lib()
     rc = lib.tg_beam_select(dev, stream, lp, ltype, g, k, v, lg, lk, sp, mp, mg, mk, fp, pad, 1 if normalize else 0, b, op, pp, tp, wp, nws)
     if rc:
