@@ -1,4 +1,4 @@
-"""Calls that need more blocks than one launch holds (2^32 threads along x), on PyTorch tensors; run in a child process by
+"""Calls that need more blocks than one launch holds (2^32 threads along x), and a captured launch, on PyTorch tensors; run in a child process by
 test_gpu_ops_launches.py.  Every case stays below 25 GB."""
 import gc
 
@@ -107,3 +107,30 @@ def test_more_items_to_reorder():
     for a, st in enumerate(states):
         for i in pieces(g * k):
             assert torch.equal(st[i], rows(src[i], a)), a
+
+
+def test_a_captured_product_reads_an_engines_buffer_at_every_replay():
+    import numpy as np
+
+    from tetris_gymnasium_amd import Engine, _native as N
+
+    e = Engine(512, 10, 20, obs_mode=N.OBS_BOARD)
+    e.reset(np.arange(1, 513, dtype=np.uint64))
+    a = e.device_array(N.BUF_OBS)
+    x = ops.DeviceView(a.ptr, a.shape, "uint8")  # (the array itself would wait for its engine inside the capture)
+    w = torch.randint(-127, 128, (16, 10), device="cuda", dtype=torch.int32).to(torch.int8)
+    y, one = torch.empty(512, 20, 16, device="cuda"), torch.ones(16, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    e.sync()
+    with torch.cuda.graph(graph):
+        ops.linear_i8(x, w, one, y, stream=stream())
+    r = np.random.default_rng(0)
+    for _ in range(4):
+        for _ in range(9):
+            e.step_async(r.integers(0, 8, 512))
+        e.sync()
+        graph.replay()
+        torch.cuda.synchronize()
+        obs = torch.from_numpy(e.observation()).float()
+        assert torch.equal(y.cpu(), obs @ w.cpu().float().T)
+    e.close()

@@ -112,3 +112,22 @@ def test_the_search_outlives_games_at_random():
         over |= e.step(e.sample_legal_actions(seed=5, counter=t))[1] != 0
     assert over.any()  # (the search ends none of the eight in 40 placements)
     e.close()
+
+
+def test_reorder_beams_of_an_engine_on_several_streams():
+    B, K = 32768, 8
+    r = np.random.default_rng(0)
+    engines = [Engine(B, 10, 20, obs_mode=N.OBS_BOARD, autoreset=N.AUTORESET_SAME_STEP, streams=n) for n in (1, 2)]
+    for e in engines:
+        e.reset(np.arange(1, B + 1, dtype=np.uint64))
+    for t in range(24):
+        a, p = r.integers(0, 8, B).astype(np.int32), r.integers(-1, K, (B // K, K)).astype(np.int32)
+        for e in engines:
+            e.step_async(a)
+            if t % 3 == 2:
+                e.reorder_beams(p, K)
+    for x, y in zip(*(e.get_state() for e in engines)):
+        np.testing.assert_array_equal(x, y)
+    np.testing.assert_array_equal(engines[0].observation(), engines[1].observation())
+    for e in engines:
+        e.close()

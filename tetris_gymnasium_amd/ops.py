@@ -9,7 +9,8 @@ Arrays are device memory of one GPU: a PyTorch tensor, a `DeviceArray` of an Eng
 `__cuda_array_interface__`, or a `DeviceView` around a raw pointer.  Outputs are the caller's; nothing is allocated, kept or
 waited for.  Calls run on `stream` (an integer hipStream_t, e.g. `torch.cuda.current_stream().cuda_stream`; 0 = the default
 stream) in order with whatever else runs there, and may be captured into a graph.  A `DeviceArray` is exported as to any other
-consumer: its engine's stream is waited for first.  A call runs on its arrays' device, whatever the current one is (an array that is
+consumer: its engine's stream is waited for first, which a capture does not allow: there, wait for the engine beforehand and pass a
+`DeviceView` of the array's `ptr`.  A call runs on its arrays' device, whatever the current one is (an array that is
 known by `__cuda_array_interface__` alone does not tell: that of the others, or 0).  Bad arguments raise ValueError, a failed
 call EngineError."""
 from __future__ import annotations
@@ -391,7 +392,8 @@ def _state(meta, rows, what):
 def beam_reorder(states, parents, *, out=None, beams_in=None, stream=0):
     """Rows that follow their beams: out[i][g, j] = states[i][g, parents[g, j]] for up to 24 arrays in one launch.
 
-    states: an array or a list of arrays [G * K, ...] or [G, K, ...] of any element type; parents int32 [G, B] as beam_select leaves
+    states: an array or a list of arrays [G * K, ...] or [G, K, ...] of integers or floating-point numbers of 8 to 64 bits (other types:
+    as a view of their bytes); parents int32 [G, B] as beam_select leaves
     them.  K = beams_in, by default B.  out: the same number of arrays with B rows per group (not overlapping states), or None to
     reorder in place (B = K).
     A parent outside 0 .. K - 1 (the -1 of a missing beam) leaves its row as it was.  Returns out (or states)."""
