@@ -171,7 +171,7 @@ template <int N, class F> __device__ __forceinline__ int wave_top(const Cand (&k
 
 // Small searches: a wave per group, L = the power of two below 64 / K lanes per beam, N entries per lane (V <= L * N).  The log-sum of
 // a beam is a reduction over its L lanes.  Everything stays in registers; the input is read once.  Bound by vector instructions: 8 192
-// groups x 8 beams x 40 entries in f32 under a mask (13 MB) 11.7 us at 558 of them per wave, 8 us without log-probabilities; one group 2.6 us.
+// groups x 8 beams x 40 entries in f32 under a mask (13 MB) 11.8 us at 567 of them per wave, 8 us without log-probabilities; one group 2.6 us.
 template <class T, int N> __global__ __launch_bounds__(256) void select_small_kernel(const SelectArgs a, int shift) {
   __shared__ Cand lds[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -243,7 +243,7 @@ template <class T, int N> __global__ __launch_bounds__(256) void select_small_ke
 
 // Large searches, first step: a workgroup per (beam, chunk of 256 * E entries), the chunk in registers: its maximum, its sum of
 // exponentials against that maximum, and its best `beams` entries by (logit, place).  32 x 8 x 32 768 in bf16 (17 MB): 14.5 us, 7 of them
-// the issue of 944 vector instructions per wave (5 us without the exponentials, 3 without the list); chunks of 4 096: 15.0, 2 048: 18.0.
+// the issue of 943 vector instructions per wave (5 us without the exponentials, 3 without the list); chunks of 4 096: 15.0, 2 048: 18.0.
 // What reaches a wave's bound is ranked by counting, so the list is kept short: where many equal logits (a clipped or a constant row), rising
 // ones or many beams bring more than kSelectList entries, every wave first narrows its bound until at most kSelectWave remain.
 // 32 x 8 x 32 768 in bf16, whole calls at 8, 16, 64 beams: random logits 20, 37, 114 us, all equal 44, 53, 363 (ranking the
@@ -528,8 +528,8 @@ inline SelectPlan select_plan(int64_t groups, int64_t k, int64_t v) {
 // An item is gp groups x kout beams x cb columns (units of 1 << shift bytes) of one array, at most 64 * kReorderReg units: a wave takes
 // the whole item into registers before it stores any of it, and columns of a row do not depend on each other, so the rows of a
 // group may be permuted in place.  Rows go in units of 16 bytes at whatever address they start, and what is left of them (below 16
-// bytes) as an array of its own.  Bound by memory: 65 536 envs of 320 bytes in four arrays (42 MB) 10.4 us = 4.0 TB/s (in
-// units of 8 bytes 11.4), 32 rows of 1 MiB (67 MB) 12.7 us = 5.3 TB/s, in place 9.8.
+// bytes) as an array of its own.  Bound by memory: 65 536 envs of 320 bytes in four arrays (42 MB) 10.5 us = 4.0 TB/s (in
+// units of 8 bytes 11.4), 32 rows of 1 MiB (67 MB) 13.0 us = 5.2 TB/s; in place, whole calls, 9.8 and 10.7.
 constexpr int kReorderReg = 8, kReorderMax = 48;
 struct ReorderArray {
   const uint8_t* src;

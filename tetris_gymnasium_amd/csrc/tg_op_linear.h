@@ -107,8 +107,8 @@ template <class OT, int N> __device__ __forceinline__ void linear_store(const Li
 // ---- short rows (K <= 64 * KS), many of them ------------------------------------------------------------------------------------
 // Bound by memory: a byte of input is used N times, N <= a few hundred.  A wave keeps the weights of 64 columns in registers (16 KS
 // of them) and walks over tiles of 16 rows, the next tile's fragments in flight behind the present one's products.  65 536 boards of
-// 200 bytes into 256 bf16 (47 MB): 16.1 us = 2.9 TB/s, 7.7 of them until the first tile is out; without its stores 12, without
-// loads and stores 11.  Two or three tiles in flight, or three workgroups per unit, are not faster.
+// 200 bytes into 256 bf16 (47 MB): 16.3 us = 2.9 TB/s, 7.7 of them until the first tile is out; without its stores 12, without
+// loads and stores 11: 2 023 vector instructions a wave at two waves a SIMD are 6 - 7 us of issue.  Two or three tiles in flight, or three workgroups per unit, are not faster.
 template <class OT, bool U8, int KS> __global__ __launch_bounds__(256) void linear_rows_kernel(const LinearArgs a, int shift, int64_t inside) {
   // C columns make 16 bytes of output, G tiles a lane's C columns: the four lanes of a row then store 64 bytes side by side at a time
   constexpr int C = 16 / (int)sizeof(OT), G = C / 4;
@@ -145,7 +145,7 @@ template <class OT, bool U8, int KS> __global__ __launch_bounds__(256) void line
   }
   const bool wide = n0 + 64 <= a.n;
   struct alignas(8) Column { float ws, b; };
-  __shared__ Column column[4][64];  // of each wave's strip: 32 registers less, a third wave per SIMD
+  __shared__ Column column[4][64];  // of each wave's strip: 32 registers less (up to K = 128 a third wave per SIMD; above, 180 - 200: two)
   {
     const int64_t c = n0 + lane < a.n ? n0 + lane : a.n - 1;
     column[wave][lane] = {a.ws[c], a.bias ? a.bias[c] : 0.0f};
@@ -298,8 +298,8 @@ template <class OT, bool U8, int T, int U> __global__ __launch_bounds__(512) voi
 // counted).  ALIGNED (16-byte addresses throughout): the tiles go from memory to LDS without passing registers.  32 x 32 x 32 products;
 // the LDS row d of the weights holds column 16 (d >> 2 & 1) + 4 (d >> 3) + (d & 3) of its 32, so that a lane ends with sixteen consecutive
 // columns of one row.
-// Bound by the matrix units' power: 8 192 x 4 096 x 4 096 with random bytes runs at 1.9 - 2.0 PFLOP/s (138 - 150 us), the products alone,
-// without loads, LDS reads and barriers, at 2.2 - 2.5, and the same kernel on zeros at 2.3.  64 bytes of K in three to five stages were
+// Bound by the matrix units' power: 8 192 x 4 096 x 4 096 with random bytes runs at 1.67 - 2.02 POP/s (156 - 164 us at the median, 136 at best), the
+// products alone, without loads, LDS reads and barriers, at 2.2 - 2.6, and the same kernel on zeros at 2.3.  64 bytes of K in three to five stages were
 // slower (150 - 168 us: half lines), tiles of 256 x 128 and 128 x 128 too (165, 162 us: more loads), four waves of 128 x 128 too (167 us).
 __device__ const v4i kZero16 = {0, 0, 0, 0};
 

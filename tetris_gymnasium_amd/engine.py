@@ -533,7 +533,8 @@ class Engine:
         """Env g * beams + j becomes a copy of env g * beams + parents[g, j] in every respect — board, record, generator, observation,
         last outputs, episode statistics —, in place and asynchronous (tg_reorder_beams).  parents: int32 device memory of `batch`
         entries (an integer pointer, a DeviceBuffer or any device array, as ops.beam_select leaves it, written in order with the
-        engine's stream) or a host array; an entry outside 0 .. beams - 1 leaves its env alone."""
+        engine's stream) or a host array; an entry outside 0 .. beams - 1 leaves its env alone.  Actions drawn before
+        (sample_legal_actions) are not moved: draw again."""
         self._need_ops()
         beams = int(beams)
         if beams < 1 or self.B % beams:

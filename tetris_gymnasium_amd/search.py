@@ -77,7 +77,9 @@ class PlacementScorer:
 class BeamSearch:
     """`beams` parallel continuations for every env of `engine` (NUMPY rules, stock mappings or its own), on a second engine of
     batch * beams environments next to it; `engine` itself is only read.  plan() may be called any number of times.  States are searched as
-    they are, without resets: for an env whose game is over, what a plan says is of no use."""
+    they are, without resets: for an env whose game is over, what a plan says is of no use.  The search steps copies of the
+    environments with their generators, so it knows every piece to come, also behind the visible queue: its returns are not those of a
+    policy that sees the observation alone."""
 
     def __init__(self, engine: Engine, scorer: PlacementScorer, beams=8):
         if engine.ruleset != N.RULESET_NUMPY:
